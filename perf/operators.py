@@ -1,0 +1,447 @@
+"""Cases that time the operators of sparse routing: routing to experts, the experts' products, the combination of
+their results, and low-rank adapters of many requests.
+
+Every case is one call as a mixture-of-experts layer or a server with many adapters makes it.  `run` computes it in
+elementary torch operations, or through `mergepath_spmm_amd.routing` where `own` is set; `exact` computes the same from
+the definition in 64 bits.
+
+The routing matrix of T tokens, with k nonzeros in every row, is held by its rows (expert[T, k], weight[T, k]) and by
+its columns: expert_ptr[E + 1], the slots t * k + j in the order of their experts (those without an expert, marked -1,
+behind all others), and the place pos[T, k] of each slot in that order (-1 where it has none).
+"""
+import math
+
+import torch
+
+own = False
+
+_TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+_BYTES = {"f32": 4, "f16": 2, "bf16": 2}
+
+
+def _routing():
+    from __graft_entry__ import load_package
+    return load_package().routing
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Cases
+# ---------------------------------------------------------------------------------------------------------------------
+
+def listed():
+    sigmoid = {"score": "sigmoid", "bias": True, "groups": 8, "top_groups": 4, "group_score": "top2", "renormalise": True,
+               "scale": 2.5}
+    softmax = {"score": "softmax", "bias": False, "groups": 1, "top_groups": 1, "group_score": "max", "renormalise": False,
+               "scale": 1.0}
+    return [
+        # one decoding step of a few requests: launches and latency are all there is
+        {"name": "route, 4 tokens", "op": "route", "T": 4, "E": 256, "k": 8, "type": "f32", **sigmoid},
+        # a batch of prompts through the gate of a layer with many small experts
+        {"name": "route, 16384 tokens", "op": "route", "T": 16384, "E": 256, "k": 8, "type": "f32", **sigmoid},
+        # the gate's gradient in a training step, with a number of tokens and of experts that fills no tile
+        {"name": "route backward, odd", "op": "route_backward", "T": 8191, "E": 72, "k": 6, "type": "f16", **softmax},
+        # decoding: every expert has a few rows, so the weights' bytes are the time
+        {"name": "experts, decoding", "op": "experts", "T": 32, "E": 64, "k": 6, "K": 2048, "N": 1024, "type": "bf16",
+         "gather": True},
+        # prompts: long and ragged segments, compute bound; N is no multiple of 256
+        {"name": "experts, prompts", "op": "experts", "T": 8192, "E": 64, "k": 6, "K": 2048, "N": 1408, "type": "f16",
+         "gather": True},
+        # single precision, with rows of no whole 16 bytes, in the second product (rows already in the experts' order)
+        {"name": "experts, fp32 odd", "op": "experts", "T": 1001, "E": 12, "k": 2, "K": 333, "N": 517, "type": "f32",
+         "gather": False},
+        # the two gradients of a training step
+        {"name": "experts, gradient of rows", "op": "experts_dx", "T": 8192, "E": 32, "k": 4, "K": 2048, "N": 1024,
+         "type": "bf16", "gather": True},
+        {"name": "experts, gradient of weights", "op": "experts_dw", "T": 8192, "E": 32, "k": 4, "K": 2048, "N": 1024,
+         "type": "bf16", "gather": True},
+        # the experts' rows of every token weighted and added; some slots have no expert
+        {"name": "combine", "op": "combine", "T": 8192, "E": 64, "k": 6, "N": 2048, "type": "bf16", "none": 0.05},
+        {"name": "combine backward", "op": "combine_backward", "T": 4099, "E": 64, "k": 8, "N": 1030, "type": "f16",
+         "none": 0.05},
+        # decoding for requests with adapters of their own, beside the shared projection's result
+        {"name": "adapters, decoding", "op": "adapters", "T": 64, "E": 48, "R": 16, "K": 4096, "N": 4096, "type": "bf16",
+         "none": 0.1},
+        # prompts of requests with adapters
+        {"name": "adapters, prompts", "op": "adapters", "T": 8192, "E": 12, "R": 64, "K": 4096, "N": 4096, "type": "f16",
+         "none": 0.1},
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 0.5)))))))
+
+
+def draw(rng):
+    op = rng.choice(["route", "route", "route_backward", "experts", "experts", "experts_dx", "experts_dw", "combine",
+                     "combine_backward", "adapters", "adapters"])
+    kind = rng.choice(["f32", "f16", "bf16"])
+    if op in ("route", "route_backward"):
+        groups = rng.choice([1, 1, 2, 4, 8])
+        size = _log(rng, 4, 512 // groups if groups > 1 else 400)
+        E = groups * size
+        top_groups = rng.randint(1, groups)
+        k = rng.randint(1, min(16, top_groups * size))
+        return {"op": op, "T": _log(rng, 1, min(16384, 4194304 // E)), "E": E, "k": k, "type": kind,
+                "score": rng.choice(["sigmoid", "softmax"]), "bias": rng.random() < 0.5, "groups": groups,
+                "top_groups": top_groups, "group_score": rng.choice(["max", "top2"]), "renormalise": rng.random() < 0.6,
+                "scale": rng.choice([1.0, 2.5])}
+    if op in ("combine", "combine_backward"):
+        E, k, N = _log(rng, 2, 128), 0, _log(rng, 16, 4096)
+        k = rng.randint(1, min(8, E))
+        N = N if rng.random() < 0.3 else (N + 7) // 8 * 8
+        return {"op": op, "T": _log(rng, 1, max(1, min(16384, 48 * 1024 * 1024 // (N * k)))), "E": E, "k": k, "N": N,
+                "type": kind, "none": rng.choice([0.0, 0.05, 0.3])}
+    K, N = _log(rng, 64, 4096), _log(rng, 64, 4096)
+    if rng.random() < 0.7:
+        K, N = (K + 31) // 32 * 32, (N + 31) // 32 * 32
+    if op == "adapters":
+        E, R = _log(rng, 1, 64), rng.choice([4, 8, 16, 24, 32, 64])
+        most = 8192 * 4096 // max(K, N, 512)
+        return {"op": op, "T": _log(rng, 1, min(8192, most)), "E": E, "R": R, "K": K, "N": N, "type": kind,
+                "none": rng.choice([0.0, 0.1, 0.5])}
+    E = _log(rng, 2, min(128, max(2, 200 * 1024 * 1024 // (K * N))))
+    k = rng.randint(1, min(8, E))
+    most = 8192 * 6 * 2048 * 1408 // (K * N * k * (4 if kind == "f32" else 1))
+    return {"op": op, "T": _log(rng, 1, max(1, min(8192, most))), "E": E, "k": k, "K": K, "N": N, "type": kind,
+            "gather": rng.random() < 0.5}
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Inputs
+# ---------------------------------------------------------------------------------------------------------------------
+
+def _ids(g, T, E, k, none):
+    """Distinct experts for every token, some experts more popular than others; -1 with probability `none`."""
+    liked = torch.randn(T, E, generator=g, device="cuda") + 0.5 * torch.randn(E, generator=g, device="cuda")
+    expert = liked.topk(k, dim=1).indices.int()
+    if none:
+        expert = torch.where(torch.rand(T, k, generator=g, device="cuda") < none, expert.new_full((), -1), expert)
+    return expert
+
+
+def _columns(expert, E):
+    """The routing matrix by its columns, from torch's stable sort."""
+    flat = expert.reshape(-1)
+    key = torch.where(flat < 0, torch.full_like(flat, E), flat)
+    slot = torch.sort(key, stable=True).indices
+    count = (key[:, None] == torch.arange(E, device="cuda")).sum(0)
+    expert_ptr = torch.cat([count.new_zeros(1), count.cumsum(0)])
+    pos = torch.empty_like(slot)
+    pos[slot] = torch.arange(slot.numel(), device="cuda")
+    pos = torch.where(flat < 0, pos.new_full((), -1), pos).view_as(expert)
+    return expert_ptr.int(), slot.int(), pos.int(), int(count.max())
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    t = _TYPES[case["type"]]
+
+    def normal(*shape, scale=1.0):
+        return (torch.randn(*shape, generator=g, device="cuda") * scale).to(t)
+
+    s = {"case": case}
+    T, E = case["T"], case["E"]
+    if case["op"] in ("route", "route_backward"):
+        s["scores"] = normal(T, E, scale=1.5)
+        s["bias"] = torch.randn(E, generator=g, device="cuda") * 0.05 if case["bias"] else None
+        if case["op"] == "route_backward":
+            expert, _ = _choose(s["scores"], s["bias"], case)
+            s["expert"] = expert.int()
+            s["dweight"] = torch.randn(T, case["k"], generator=g, device="cuda")
+        return s
+    k = case.get("k", 1)
+    s["expert"] = _ids(g, T, E, k, case.get("none", 0.0))
+    s["expert_ptr"], s["slot"], s["pos"], s["most"] = _columns(s["expert"], E)
+    if case["op"] == "adapters":
+        s["X"], s["base"] = normal(T, case["K"]), normal(T, case["N"])
+        s["A"] = normal(E, case["R"], case["K"], scale=case["K"] ** -0.5)
+        s["B"] = normal(E, case["N"], case["R"], scale=case["R"] ** -0.5)
+        s["scale"] = 0.5 + torch.rand(E, generator=g, device="cuda")
+    elif case["op"] in ("combine", "combine_backward"):
+        s["Z"] = normal(T * k, case["N"])
+        s["weight"] = torch.rand(T, k, generator=g, device="cuda") * (2.0 / k)
+        if case["op"] == "combine_backward":
+            s["dY"] = normal(T, case["N"])
+    else:
+        K, N = case["K"], case["N"]
+        if case["op"] != "experts_dx":
+            s["X"] = normal(T if case["gather"] else T * k, K)
+        if case["op"] != "experts_dw":
+            s["W"] = normal(E, N, K, scale=K ** -0.5)
+        if case["op"] != "experts":
+            s["dY"] = normal(T * k, N)
+    return s
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# One pass
+# ---------------------------------------------------------------------------------------------------------------------
+
+def _options(case):
+    return {m: case[m] for m in ("score", "groups", "top_groups", "group_score", "renormalise", "scale")}
+
+
+def run(s):
+    case = s["case"]
+    op = case["op"]
+    if own:
+        return _run_own(s, case, op)
+    if op == "route":
+        return _route(s["scores"], s["bias"], case)
+    if op == "route_backward":
+        return _route_backward(s["scores"], s["expert"], s["dweight"], case)
+    if op == "combine":
+        return _combine(s)
+    if op == "combine_backward":
+        return _combine_backward(s)
+    if op == "adapters":
+        return _adapters(s)
+    return _experts(s, case, op)
+
+
+def _run_own(s, case, op):
+    r = _routing()
+    if op == "route":
+        m = r.route(s["scores"], case["k"], bias=s["bias"], **_options(case))
+        return {"expert": m.expert, "weight": m.weight, "expert_ptr": m.expert_ptr, "slot": m.slot, "pos": m.pos}
+    if op == "route_backward":
+        return r.route_backward(s["scores"], s["expert"], s["dweight"], score=case["score"], renormalise=case["renormalise"],
+                                scale=case["scale"])
+    if op == "combine":
+        return r.combine(s["Z"], s["pos"], s["weight"])
+    if op == "combine_backward":
+        return r.combine_backward(s["dY"], s["Z"], s["pos"], s["weight"])
+    if op == "adapters":
+        return r.adapters_mm(s["X"], s["A"], s["B"], s["scale"], s["expert_ptr"], s["slot"], base=s["base"])
+    slot, k = (s["slot"], case["k"]) if case["gather"] else (None, 1)
+    if op == "experts":
+        return r.experts_mm(s["X"], s["W"], s["expert_ptr"], slot=slot, k=k)
+    if op == "experts_dx":
+        return r.experts_mm_dx(s["dY"], s["W"], s["expert_ptr"])
+    return r.experts_mm_dw(s["dY"], s["X"], s["expert_ptr"], slot=slot, k=k)
+
+
+def _score(scores, case):
+    """Scores in 64 bits: the choice next to a border must not hang on the rounding of exp."""
+    l = scores.double()
+    if case["score"] == "sigmoid":
+        return 1.0 / (1.0 + torch.exp(-l))
+    p = torch.exp(l - l.amax(1, keepdim=True))
+    return p / p.sum(1, keepdim=True)
+
+
+def _choose(scores, bias, case):
+    T, E = scores.shape
+    s = _score(scores, case)
+    c = s if bias is None else s + bias.double()
+    if case["groups"] > 1:
+        c = c.view(T, case["groups"], -1)
+        of_group = c.amax(2) if case["group_score"] == "max" else torch.sort(c, dim=2, descending=True).values[:, :, :2].sum(2)
+        kept = torch.sort(of_group, dim=1, descending=True, stable=True).indices[:, :case["top_groups"]]
+        keep = torch.zeros_like(of_group, dtype=torch.bool).scatter_(1, kept, True)
+        c = c.masked_fill(~keep[:, :, None], -math.inf).reshape(T, E)
+    expert = torch.sort(c, dim=1, descending=True, stable=True).indices[:, :case["k"]]
+    return expert, s
+
+
+def _route(scores, bias, case):
+    T, E = scores.shape
+    expert, s = _choose(scores, bias, case)
+    w = s.gather(1, expert)
+    if case["renormalise"]:
+        w = w / w.sum(1, keepdim=True)
+    w = (w * case["scale"]).float()
+    flat = expert.reshape(-1)
+    slot = torch.sort(flat, stable=True).indices
+    count = torch.zeros(E, dtype=torch.int64, device=flat.device).index_add_(0, flat, torch.ones_like(flat))
+    expert_ptr = torch.cat([count.new_zeros(1), count.cumsum(0)])
+    pos = torch.empty_like(slot)
+    pos[slot] = torch.arange(slot.numel(), device=slot.device)
+    return {"expert": expert.int(), "weight": w, "expert_ptr": expert_ptr.int(), "slot": slot.int(),
+            "pos": pos.view_as(expert).int()}
+
+
+def _route_backward(scores, expert, dweight, case):
+    l, at = scores.float(), expert.long()
+    if case["score"] == "sigmoid":
+        s = 1.0 / (1.0 + torch.exp(-l))
+    else:
+        p = torch.exp(l - l.amax(1, keepdim=True))
+        s = p / p.sum(1, keepdim=True)
+    chosen = s.gather(1, at)
+    d = dweight * case["scale"]
+    if case["renormalise"]:
+        total = chosen.sum(1, keepdim=True)
+        d = (d - (d * chosen / total).sum(1, keepdim=True)) / total
+    ds = torch.zeros_like(l).scatter_(1, at, d)
+    dl = ds * s * (1.0 - s) if case["score"] == "sigmoid" else s * (ds - (ds * s).sum(1, keepdim=True))
+    return dl.to(scores.dtype)
+
+
+def _padded(s, E):
+    """Places of the experts' rows in a batch with as many rows for each expert as the longest has."""
+    ptr = s["expert_ptr"].long()
+    place = ptr[:-1, None] + torch.arange(s["most"], device="cuda")
+    real = place < ptr[1:, None]
+    place = place.clamp(max=s["slot"].numel() - 1)
+    row = torch.arange(s["slot"].numel(), device="cuda")
+    of = (torch.searchsorted(ptr, row, right=True) - 1).clamp(max=E - 1)
+    return place, real, of, (row - ptr[of]).clamp(max=s["most"] - 1)
+
+
+def _experts(s, case, op):
+    place, real, of, within = _padded(s, case["E"])
+    if op != "experts_dx":
+        X = s["X"].float()[s["slot"].long()[place] // case["k"] if case["gather"] else place]
+    if op == "experts":
+        return torch.matmul(X, s["W"].float().transpose(1, 2))[of, within].to(s["X"].dtype)
+    dY = s["dY"].float()[place]
+    if op == "experts_dx":
+        return torch.matmul(dY, s["W"].float())[of, within].to(s["dY"].dtype)
+    return torch.matmul((dY * real[:, :, None]).transpose(1, 2), X).to(s["dY"].dtype)
+
+
+def _combine(s):
+    pos = s["pos"].long()
+    rows = s["Z"].float()[pos.clamp(min=0)]
+    w = torch.where(pos < 0, 0.0, s["weight"])
+    return (rows * w[:, :, None]).sum(1).to(s["Z"].dtype)
+
+
+def _combine_backward(s):
+    pos = s["pos"].long()
+    rows, dY = s["Z"].float()[pos.clamp(min=0)], s["dY"].float()
+    dweight = torch.where(pos < 0, 0.0, (rows * dY[:, None, :]).sum(2))
+    dZ = torch.zeros(s["Z"].shape, device="cuda")
+    token = torch.div(s["slot"].long(), pos.shape[1], rounding_mode="floor")
+    routed = torch.arange(s["slot"].numel(), device="cuda") < s["expert_ptr"][-1]
+    dZ = torch.where(routed[:, None], dY[token] * s["weight"].reshape(-1)[s["slot"].long()][:, None], dZ)
+    return {"dZ": dZ.to(s["Z"].dtype), "dweight": dweight}
+
+
+def _adapters(s):
+    E = s["A"].shape[0]
+    place, real, of, within = _padded(s, E)
+    row = s["slot"].long()
+    V = torch.matmul(s["X"].float()[row[place]], s["A"].float().transpose(1, 2))
+    D = torch.matmul(V, s["B"].float().transpose(1, 2)) * s["scale"][:, None, None]
+    routed = torch.arange(row.numel(), device="cuda") < s["expert_ptr"][-1]
+    delta = torch.empty(s["base"].shape, device="cuda")
+    delta[row] = torch.where(routed[:, None], D[of, within], 0.0)
+    return (s["base"].float() + delta).to(s["base"].dtype)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# What a pass cannot do without
+# ---------------------------------------------------------------------------------------------------------------------
+
+def work(case):
+    T, E, b = case["T"], case["E"], _BYTES[case["type"]]
+    k = case.get("k", 1)
+    M = T * k
+    met = E * (1.0 - (1.0 - k / E) ** T)  # experts that have a row, expected
+    if case["op"] == "route":
+        return {"bytes": T * E * b + (4 * E if case["bias"] else 0) + 16 * M + 4 * (E + 1), "flops": 0}
+    if case["op"] == "route_backward":
+        return {"bytes": 2 * T * E * b + 8 * M, "flops": 0}
+    routed = M * (1.0 - case.get("none", 0.0))
+    if case["op"] == "combine":
+        return {"bytes": (routed + T) * case["N"] * b + 8 * M, "flops": 2 * routed * case["N"]}
+    if case["op"] == "combine_backward":
+        return {"bytes": (routed + M + T) * case["N"] * b + 12 * M, "flops": 3 * routed * case["N"]}
+    K, N = case["K"], case["N"]
+    if case["op"] == "adapters":
+        R = case["R"]
+        return {"bytes": (T * K + 2 * T * N + met * R * (K + N)) * b + 4 * T, "flops": 2 * routed * R * (K + N)}
+    rows = (T if case["gather"] and case["op"] != "experts_dx" else M) * (K if case["op"] != "experts_dx" else N)
+    if case["op"] == "experts_dw":
+        return {"bytes": (rows + M * N + E * N * K) * b + 4 * M, "flops": 2 * M * N * K}
+    return {"bytes": (rows + M * (N if case["op"] == "experts" else K) + met * N * K) * b + 4 * M, "flops": 2 * M * N * K}
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# The definitions in 64 bits
+# ---------------------------------------------------------------------------------------------------------------------
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    op = case["op"]
+    if op in ("route", "route_backward"):
+        return _exact_route(s, case)
+    d = {m: v.double() for m, v in s.items() if isinstance(v, torch.Tensor) and v.is_floating_point()}
+    ptr, slot, pos = s["expert_ptr"].tolist(), s["slot"].long(), s["pos"].long()
+    T, E, k = case["T"], case["E"], case.get("k", 1)
+    if op == "combine":
+        Y = torch.zeros(T, case["N"], dtype=torch.float64, device="cuda")
+        for j in range(k):
+            has = pos[:, j] >= 0
+            Y[has] += d["weight"][has, j, None] * d["Z"][pos[has, j]]
+        return Y
+    if op == "combine_backward":
+        dZ, dweight = torch.zeros_like(d["Z"]), torch.zeros_like(d["weight"])
+        for j in range(k):
+            has = pos[:, j] >= 0
+            dZ[pos[has, j]] = d["weight"][has, j, None] * d["dY"][has]
+            dweight[has, j] = (d["Z"][pos[has, j]] * d["dY"][has]).sum(1)
+        return {"dZ": dZ, "dweight": dweight}
+    if op == "adapters":
+        Y = d["base"].clone()
+        for e in range(E):
+            rows = slot[ptr[e]:ptr[e + 1]]
+            Y[rows] += d["scale"][e] * ((d["X"][rows] @ d["A"][e].t()) @ d["B"][e].t())
+        return Y
+    N, K = case["N"], case["K"]
+    out = torch.zeros((E, N, K) if op == "experts_dw" else (T * k, N if op == "experts" else K), dtype=torch.float64,
+                      device="cuda")
+    for e in range(E):
+        a, b = ptr[e], ptr[e + 1]
+        if op != "experts_dx":
+            X = d["X"][torch.div(slot[a:b], k, rounding_mode="floor")] if case["gather"] else d["X"][a:b]
+        if op == "experts":
+            out[a:b] = X @ d["W"][e].t()
+        elif op == "experts_dx":
+            out[a:b] = d["dY"][a:b] @ d["W"][e]
+        else:
+            out[e] = d["dY"][a:b].t() @ X
+    return out
+
+
+def _exact_route(s, case):
+    """Greedy, one expert after the other, as the definition says it; the gradient is that of autograd."""
+    l = s["scores"].double().requires_grad_(case["op"] == "route_backward")
+    p = torch.sigmoid(l) if case["score"] == "sigmoid" else torch.softmax(l, 1)
+    T, E, k = case["T"], case["E"], case["k"]
+
+    def first_largest(v):
+        return (v == v.amax(1, keepdim=True)).to(torch.uint8).argmax(1)
+
+    if case["op"] == "route":
+        open_ = p.clone() if s["bias"] is None else p + s["bias"].double()
+        if case["groups"] > 1:
+            members = open_.view(T, case["groups"], E // case["groups"])
+            of_group = members.amax(2)
+            if case["group_score"] == "top2":
+                of_group = members.topk(2, dim=2).values.sum(2)
+            shut = torch.ones_like(of_group, dtype=torch.bool)
+            for _ in range(case["top_groups"]):
+                best = first_largest(of_group)[:, None]
+                shut.scatter_(1, best, False)
+                of_group.scatter_(1, best, -math.inf)
+            open_ = open_.masked_fill(shut.repeat_interleave(E // case["groups"], 1), -math.inf)
+        columns = []
+        for _ in range(k):
+            best = first_largest(open_)[:, None]
+            columns.append(best)
+            open_ = open_.scatter(1, best, -math.inf)
+        expert = torch.cat(columns, 1)
+    else:
+        expert = s["expert"].long()
+    w = p.gather(1, expert)
+    if case["renormalise"]:
+        w = w / w.sum(1, keepdim=True)
+    w = w * case["scale"]
+    if case["op"] == "route_backward":
+        w.backward(s["dweight"].double())
+        return l.grad
+    expert_ptr, slot, pos, _ = _columns(expert, E)
+    return {"expert": expert.int(), "weight": w, "expert_ptr": expert_ptr, "slot": slot, "pos": pos}
