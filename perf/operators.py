@@ -210,7 +210,7 @@ def _run_own(s, case, op):
     if op == "combine":
         return r.combine(s["Z"], s["pos"], s["weight"])
     if op == "combine_backward":
-        return r.combine_backward(s["dY"], s["Z"], s["pos"], s["weight"])
+        return r.combine_backward(s["dY"], s["Z"], s["weight"], s["expert_ptr"], s["slot"])
     if op == "adapters":
         return r.adapters_mm(s["X"], s["A"], s["B"], s["scale"], s["expert_ptr"], s["slot"], base=s["base"])
     slot, k = (s["slot"], case["k"]) if case["gather"] else (None, 1)
