@@ -625,6 +625,127 @@ int mps_nzsplit_spmm_f32(const int *d_col_idx, const float *d_val, const float *
                          float *d_Y, int n_rows, int nnz, int K, const int *d_part_ptr,
                          const int *d_part2node, int num_parts, void *stream);
 
+/* ------------------------------------------------------------------------ */
+/* Device side: sparse routing (experts and adapters of language models)     */
+/* ------------------------------------------------------------------------ */
+
+/* No counterpart in the reference.  A routing matrix is a sparse matrix of T
+ * tokens by E experts with (at most) k nonzeros in every row.  It is held
+ *   by rows     d_expert int[T * k]: the expert of slot t * k + j, -1 = none;
+ *               d_weight float[T * k]: its value, 0 where there is none;
+ *   by columns  d_expert_ptr int[E + 1]: expert e owns the places
+ *               [d_expert_ptr[e], d_expert_ptr[e + 1]);
+ *               d_slot int[T * k]: the slot at every place, ascending within
+ *               an expert; slots without an expert follow behind
+ *               d_expert_ptr[E], ascending too;
+ *               d_pos int[T * k]: the place of every slot, -1 where the slot
+ *               has no expert.
+ * Conventions beside those at the top of this file: dense data may be fp32,
+ * fp16 or bf16 (mps_dtype) and needs only its natural alignment (16-byte
+ * aligned matrices with rows of whole 16 bytes are faster); sums are held in
+ * fp32 and rounded once; calls only launch kernels (no allocation, copy,
+ * memset or synchronisation), so they can be captured; results are the same
+ * bits from run to run (no atomics on results).  Every index that a kernel
+ * reads (experts, slots, places) is checked there: one out of range counts as
+ * "none".  Calls that share a workspace must not overlap. */
+typedef enum mps_dtype { MPS_F32 = 0, MPS_F16 = 1, MPS_BF16 = 2 } mps_dtype;
+
+#define MPS_ROUTE_MAX_EXPERTS 1024
+#define MPS_ROUTE_MAX_K 32
+#define MPS_ROUTE_MAX_GROUPS 64
+#define MPS_SCORE_SOFTMAX 0
+#define MPS_SCORE_SIGMOID 1
+#define MPS_GROUP_MAX 0  /* a group counts as its largest choice score            */
+#define MPS_GROUP_TOP2 1 /* ... as the sum of its two largest                      */
+typedef struct mps_route_options {
+    int k;           /* experts per token, 1 .. min(E, MPS_ROUTE_MAX_K)            */
+    int score;       /* MPS_SCORE_*                                                */
+    int groups;      /* E / groups consecutive experts form a group; 0 or 1 = none */
+    int top_groups;  /* groups that a token may choose from, 1 .. groups           */
+    int group_score; /* MPS_GROUP_*                                                */
+    int renormalise; /* weights of a token add up to `scale`                       */
+    float scale;     /* factor on every weight                                     */
+} mps_route_options;
+
+/* Routing to experts.  With l = d_scores[t, :] (T x E),
+ *   s = softmax(l) over all E experts, or sigmoid(l);
+ *   c = s + d_bias (d_bias: float[E] or NULL), in the precision of 64 bits;
+ *   the top_groups groups with the largest group score stay (ties: the lower
+ *   group), and among their experts the k with the largest c are chosen
+ *   (ties: the lower expert), in descending order of c;
+ *   weight = scale * s, or scale * s / (sum of the chosen s).
+ * Without a bias c orders as l does, and l itself is compared.  An expert with
+ * l = -inf (or a bias of -inf) is never chosen; slots that find no expert hold
+ * -1 and weight 0, also where renormalised.  A NaN counts as the largest
+ * value, as does what is computed from one, so that it shows in the weights.
+ * d_expert_ptr, d_slot, d_pos: all three or all NULL (the rows alone).
+ * The workspace is needed for the columns only. */
+int mps_route_workspace_bytes(int T, int E, int k, size_t *bytes_out);
+int mps_route(const void *d_scores, int dtype, const float *d_bias, int T, int E, const mps_route_options *options,
+              int *d_expert, float *d_weight, int *d_expert_ptr, int *d_slot, int *d_pos, void *d_workspace,
+              size_t workspace_bytes, void *stream);
+
+/* The columns of a routing matrix whose rows d_expert[T, k] the caller has
+ * (adapters: k = 1 and the adapter of every token): a stable counting sort.
+ * Ids outside [0, E) count as -1.  E <= MPS_ROUTE_MAX_EXPERTS. */
+int mps_route_columns(const int *d_expert, int T, int E, int k, int *d_expert_ptr, int *d_slot, int *d_pos,
+                      void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* d_dscores[T, E] (the type of d_scores) from d_dweight[T, k], the gradient of
+ * the weights that mps_route gave for d_expert.  The choice itself has no
+ * gradient, so groups and bias do not matter here; options: k, score,
+ * renormalise and scale.  An expert named twice in a row gets both parts. */
+int mps_route_backward(const void *d_scores, int dtype, const int *d_expert, const float *d_dweight, int T, int E,
+                       const mps_route_options *options, void *d_dscores, void *stream);
+
+/* Products of the experts.  M = places; d_W: [E, N, K], one N x K matrix for
+ * every expert; the rows of d_Y stand in the order of the places:
+ *   d_Y[p, :] = d_X[row(p), :] * d_W[e]^T  for p in expert e's places.
+ * d_slot NULL: row(p) = p and d_X is [M, K].  Else row(p) = d_slot[p] / k and
+ * d_X is [M / k, K] (M a multiple of k): the rows of the tokens are gathered
+ * as they are needed.  Rows of d_Y from d_expert_ptr[E] on are left as
+ * they were. */
+int mps_experts_mm(const void *d_X, const void *d_W, void *d_Y, int dtype, const int *d_expert_ptr, const int *d_slot,
+                   int k, int M, int E, int N, int K, void *stream);
+/* Gradient of the rows: d_dX[p, :] = d_dY[p, :] * d_W[e], [M, K] in the order of
+ * the places (rows from d_expert_ptr[E] on are left as they were); the
+ * gradient of gathered tokens is mps_combine of it with unit weights. */
+int mps_experts_mm_dx(const void *d_dY, const void *d_W, void *d_dX, int dtype, const int *d_expert_ptr, int M, int E,
+                      int N, int K, void *stream);
+/* Gradient of the weights: d_dW[e] = sum over the places of e of
+ * d_dY[p, :]^T * d_X[row(p), :], zero for an expert without places. */
+int mps_experts_mm_dw(const void *d_dY, const void *d_X, void *d_dW, int dtype, const int *d_expert_ptr,
+                      const int *d_slot, int k, int M, int E, int N, int K, void *stream);
+
+/* Y = A * Z with the routing matrix by rows, columns given as places:
+ *   d_Y[t, :] = d_base[t, :] + sum_j d_weight[t, j] * d_Z[d_pos[t, j], :]
+ * over the slots that have a place (d_pos in [0, M)).  d_weight NULL = 1,
+ * d_base NULL = 0; d_base may be d_Y. d_Z is [M, N], d_Y [T, N]. */
+int mps_combine(const void *d_Z, const int *d_pos, const float *d_weight, const void *d_base, void *d_Y, int dtype,
+                int T, int k, int M, int N, void *stream);
+/* Its gradients, by columns: for every place p < d_expert_ptr[E] with slot
+ * s = d_slot[p], d_dZ[p, :] = d_weight[s] * d_dY[s / k, :] and
+ * d_dweight[s] = <d_dY[s / k, :], d_Z[p, :]>; zero for the places behind
+ * (their rows of d_Z are not read).  M = T * k.  d_weight NULL = 1;
+ * d_dweight may be NULL. */
+int mps_combine_backward(const void *d_dY, const void *d_Z, const float *d_weight, const int *d_expert_ptr, int E,
+                         const int *d_slot, void *d_dZ, float *d_dweight, int dtype, int T, int k, int N,
+                         void *stream);
+
+/* Low-rank adapters of many requests beside a shared projection.  Adapter a
+ * holds d_A[a] (R x K) and d_B[a] (N x R); the tokens of adapter a are
+ * d_row[d_adapter_ptr[a] .. d_adapter_ptr[a + 1]) (the columns of a routing
+ * matrix with k = 1):
+ *   d_Y[t, :] = d_base[t, :] + d_scale[a] * (d_X[t, :] * d_A[a]^T) * d_B[a]^T
+ * and d_Y[t, :] = d_base[t, :] for the tokens behind d_adapter_ptr[E].
+ * d_base NULL = 0 and may be d_Y; d_scale NULL = 1.  R <= 256.  Every token
+ * has to be in d_row once.  Workspace: mps_adapters_workspace_bytes. */
+#define MPS_ADAPTERS_MAX_RANK 256
+int mps_adapters_workspace_bytes(int T, int E, int R, int K, size_t *bytes_out);
+int mps_adapters_mm(const void *d_X, const void *d_A, const void *d_B, const float *d_scale, const void *d_base,
+                    void *d_Y, int dtype, const int *d_adapter_ptr, const int *d_row, int T, int E, int R, int K, int N,
+                    void *d_workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,8 +10,8 @@ __all__ = ["_cabi", "build", "graphs", "MpsError"]
 
 
 def __getattr__(name):
-    # spmm needs torch; load it on first use so that host-only users skip the import
-    if name == "spmm":
+    # spmm and routing need torch; load them on first use so that host-only users skip the import
+    if name in ("spmm", "routing"):
         import importlib
-        return importlib.import_module(__name__ + ".spmm")
+        return importlib.import_module(__name__ + "." + name)
     raise AttributeError(name)

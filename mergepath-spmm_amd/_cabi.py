@@ -41,6 +41,10 @@ MPS_PLAN_LOCAL_TABLES = 1024
 MPS_PLAN_NO_SWEEP = 2048
 MPS_PLAN_FORCE_SWEEP = 4096
 MPS_PLAN_HOST_BUILD = 8192
+MPS_F32, MPS_F16, MPS_BF16 = 0, 1, 2
+MPS_SCORE_SOFTMAX, MPS_SCORE_SIGMOID = 0, 1
+MPS_GROUP_MAX, MPS_GROUP_TOP2 = 0, 1
+MPS_ROUTE_MAX_EXPERTS, MPS_ROUTE_MAX_K, MPS_ROUTE_MAX_GROUPS, MPS_ADAPTERS_MAX_RANK = 1024, 32, 64, 256
 (MPS_PLAN_ARRAY_VROW_PTR, MPS_PLAN_ARRAY_COORD_X, MPS_PLAN_ARRAY_COORD_Y, MPS_PLAN_ARRAY_WAVE_OFF,
  MPS_PLAN_ARRAY_SLICE_COLS, MPS_PLAN_ARRAY_SLICE_SRC, MPS_PLAN_ARRAY_SLICE_VALS, MPS_PLAN_ARRAY_HOT_COLS,
  MPS_PLAN_ARRAY_RB_BLOCK_ROW, MPS_PLAN_ARRAY_RB_HOT_COLS, MPS_PLAN_ARRAY_RB_META, MPS_PLAN_ARRAY_RB_WAVE_BASE,
@@ -67,6 +71,12 @@ class PlanInfo(ctypes.Structure):
                [(n, ctypes.c_int) for n in ("sweep_panels", "sweep_acc_rows", "sweep_lanes", "sweep_tiles", "sweep_col_bits",
                                              "sweep_piece", "sweep_together", "sweep_split_rows", "sweep_partial_rows", "sweep_listed_rows")] + \
                [("sweep_rounds", ctypes.c_longlong), ("sweep_slots", ctypes.c_longlong), ("built_on_device", ctypes.c_int)]
+
+
+class RouteOptions(ctypes.Structure):
+    """mps_route_options (include/mpspmm.h)."""
+    _fields_ = [("k", ctypes.c_int), ("score", ctypes.c_int), ("groups", ctypes.c_int), ("top_groups", ctypes.c_int),
+                ("group_score", ctypes.c_int), ("renormalise", ctypes.c_int), ("scale", ctypes.c_float)]
 
 
 class PlanOptions(ctypes.Structure):
@@ -146,6 +156,17 @@ PROTOTYPES = {
     "mps_rowwise_bounds": (_i, [_i, _i, _vp, _vp]),
     "mps_nzsplit_max_parts": (_i, [_i, _i, _i, c_int_p]),
     "mps_nzsplit_build": (_i, [_vp, _i, _i, _vp, _vp, _i, _vp, c_int_p, _vp]),
+    "mps_route_workspace_bytes": (_i, [_i, _i, _i, ctypes.POINTER(_sz)]),
+    "mps_route": (_i, [_vp, _i, _vp, _i, _i, ctypes.POINTER(RouteOptions), _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mps_route_columns": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mps_route_backward": (_i, [_vp, _i, _vp, _vp, _i, _i, ctypes.POINTER(RouteOptions), _vp, _vp]),
+    "mps_experts_mm": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "mps_experts_mm_dx": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp]),
+    "mps_experts_mm_dw": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "mps_combine": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "mps_combine_backward": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "mps_adapters_workspace_bytes": (_i, [_i, _i, _i, _i, ctypes.POINTER(_sz)]),
+    "mps_adapters_mm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "mps_nzsplit_spmm_f32": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp]),
 }
 

@@ -1,0 +1,344 @@
+// Products of the experts: a matrix for every expert, times the rows that the
+// routing matrix sends there, with their two gradients.
+//
+// One tile kernel does all three.  A workgroup owns a 128 x 128 tile of the
+// result: P counts its columns (contiguous in memory), Q its rows,
+//   D[q, p] = sum_r Q[q, r] P[p, r],
+// with r the summed index.  An operand is stored either with r contiguous
+// (rows of 128 bytes of r are staged, one per q or p) or with p / q contiguous
+// (rows of 128 elements are staged, one per r, and turned while they are read
+// from LDS):
+//                r             P                       Q
+//   product      K             W[e], r contiguous      X, r contiguous
+//   dX           N             W[e], p contiguous      dY, r contiguous
+//   dW           places of e   X, p contiguous         dY, q contiguous
+// P is the first operand of the matrix instruction, whose result gives a lane
+// four neighbouring p of one q: stores of 8 or 16 bytes.
+#include "mpspmm_routing.hpp"
+
+namespace {
+
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef half_t half8v __attribute__((ext_vector_type(8)));
+typedef bf16_t bf16x8v __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v *lds_short4;
+
+constexpr int kTile = 128;
+constexpr int kThreads = 256;
+constexpr int kChunks = kTile * 128 / 16 / kThreads;  // 16-byte chunks of an operand's stage per thread: 4
+
+template <typename T>
+struct Elem {
+    static constexpr int kPerChunk = 16 / sizeof(T);
+    static constexpr int kDepth = 128 / sizeof(T);      // r per stage
+    static constexpr int kStep = 4 * kPerChunk;         // r per matrix step: lane group g takes chunk g
+    static constexpr int kRowChunks = kTile / kPerChunk;  // chunks of a staged row of 128 elements
+};
+
+// Where chunk c of staged row `row` lies, so that the 16 lanes that read
+// together meet 16 different chunks of the 256 bytes that LDS gives at once.
+//   r contiguous: 8 chunks a row, lanes read the same chunk of 16 rows.
+template <typename T>
+__device__ __forceinline__ int place_rows(int row, int c)
+{
+    return (row * 8 + (c ^ ((row >> 1) & 7))) * 16;
+}
+//   p / q contiguous, 16-bit: 16 chunks a row, the turning read takes 32 bytes
+//   of each of the rows 8 g + 0 .. 3 (or 4 .. 7), g = 0 .. 3; fp32: 32 chunks a
+//   row, lanes take 64 bytes of the rows 4 g + j.
+template <typename T>
+__device__ __forceinline__ int place_turned(int row, int c)
+{
+    if constexpr (sizeof(T) == 2) return (row * 16 + (c ^ (((row & 3) | ((row >> 1) & 4)) << 1))) * 16;
+    else return (row * 32 + (c ^ (((row >> 2) & 3) << 2))) * 16;
+}
+
+template <typename T>
+__device__ __forceinline__ float4v mma(uint4v p, uint4v q, float4v acc)
+{
+    if constexpr (sizeof(T) == 4) {
+        // r = 4 g + j of a step is summed by instruction j
+        const float4v a = __builtin_bit_cast(float4v, p), b = __builtin_bit_cast(float4v, q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
+        return acc;
+    } else if constexpr (__is_same(T, half_t)) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, p), __builtin_bit_cast(half8v, q), acc,
+                                                      0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, p), __builtin_bit_cast(bf16x8v, q),
+                                                       acc, 0, 0, 0);
+    }
+}
+
+// What a lane feeds to the matrix instruction for 16 neighbouring outer
+// indices from `outer` on and matrix step s.
+template <typename T, bool TURNED>
+__device__ __forceinline__ uint4v fragment(const char *stage, int outer, int s, int lane)
+{
+    const int i = lane & 15, g = lane >> 4;
+    if constexpr (!TURNED) {
+        return *reinterpret_cast<const uint4v *>(stage + place_rows<T>(outer + i, 4 * s + g));
+    } else if constexpr (sizeof(T) == 2) {
+        // 16 lanes read a block of 4 rows (r) by 16 elements, 8 bytes each, and get it turned
+        const int row = 32 * s + 8 * g + (i >> 2), c = outer / 8 + ((i & 3) >> 1), half = (i & 1) * 8;
+        union {
+            short4v part[2];
+            uint4v all;
+        } u;
+        u.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)(stage + place_turned<T>(row, c) + half));
+        u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)(stage + place_turned<T>(row + 4, c) + half));
+        return u.all;
+    } else {
+        uint4v v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            v[j] = *reinterpret_cast<const unsigned *>(stage + place_turned<T>(16 * s + 4 * g + j, (outer + i) / 4) +
+                                                       (i & 3) * 4);
+        return v;
+    }
+}
+
+// 16 bytes from p, of which `valid` elements exist; zeros for the others.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ uint4v load_chunk(const T *p, int valid)
+{
+    constexpr int V = 16 / sizeof(T);
+    uint4v v = {0, 0, 0, 0};
+    if (valid >= V) {
+        __builtin_memcpy(&v, __builtin_assume_aligned(p, ALIGNED ? 16 : sizeof(T)), 16);
+    } else if (!ALIGNED && valid > 0) {
+        T part[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) part[i] = i < valid ? p[i] : (T)0.0f;
+        __builtin_memcpy(&v, part, 16);
+    }
+    return v;
+}
+
+struct ExpertsShape {
+    int M, E, N, K, k;
+    int col_tiles, row_tiles;
+};
+
+enum Product { kForward, kRows, kWeights };
+
+template <typename T, Product WHAT, bool ALIGNED>
+__global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__restrict__ A, const T *__restrict__ B,
+                                                                   T *__restrict__ out, const int *__restrict__ ptr,
+                                                                   const int *__restrict__ slot, ExpertsShape sh)
+{
+    // product: A = X, B = W, out = Y; dX: A = dY, B = W, out = dX; dW: A = dY, B = X, out = dW
+    constexpr bool PT = WHAT != kForward, QT = WHAT == kWeights;
+    constexpr int V = Elem<T>::kPerChunk, DEPTH = Elem<T>::kDepth;
+    __shared__ __attribute__((aligned(16))) char stage_p[2][kTile * 128];
+    __shared__ __attribute__((aligned(16))) char stage_q[2][kTile * 128];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int cols = WHAT == kForward ? sh.N : sh.K;
+    const int col0 = (int)(blockIdx.x % sh.col_tiles) * kTile;
+    const int rest = blockIdx.x / sh.col_tiles;
+    int expert, row0, rows, first, depth;  // rows of the tile in the result; places summed over from `first` on
+    if constexpr (WHAT == kWeights) {
+        expert = rest / sh.row_tiles;
+        row0 = rest % sh.row_tiles * kTile;
+        rows = min(sh.N - row0, kTile);
+        first = clamp_place(ptr[expert], sh.M);
+        depth = max(clamp_place(ptr[expert + 1], sh.M) - first, 0);
+    } else {
+        const RowTile t = find_row_tile<kTile>(ptr, sh.E, sh.M, rest);
+        if (t.rows == 0) return;
+        expert = t.expert;
+        row0 = first = t.first;
+        rows = t.rows;
+        depth = WHAT == kForward ? sh.K : sh.N;
+    }
+    const T *W = WHAT == kWeights ? nullptr : B + (size_t)expert * sh.N * sh.K;
+
+    // The chunks that this thread stages.
+    const T *p_src[kChunks], *q_src[kChunks];
+    int p_valid[kChunks], q_valid[kChunks];  // turned: elements from the chunk's column on; else unused (row given or null)
+#pragma unroll
+    for (int n = 0; n < kChunks; ++n) {
+        const int id = tid + n * kThreads;
+        if constexpr (PT) {
+            const int c = id % Elem<T>::kRowChunks;
+            p_src[n] = (WHAT == kRows ? W : B) + col0 + c * V;
+            p_valid[n] = cols - (col0 + c * V);
+        } else {
+            const int row = id / 8;
+            p_src[n] = col0 + row < cols ? W + (size_t)(col0 + row) * sh.K : nullptr;
+        }
+        if constexpr (QT) {
+            const int c = id % Elem<T>::kRowChunks;
+            q_src[n] = A + row0 + c * V;
+            q_valid[n] = sh.N - (row0 + c * V);
+        } else {
+            const int row = id / 8;
+            q_src[n] = nullptr;
+            if (row < rows) {
+                int from = first + row;
+                if (WHAT == kForward && slot) {
+                    const int s = slot[from];
+                    from = (unsigned)s < (unsigned)sh.M ? s / sh.k : -1;
+                }
+                if (from >= 0) q_src[n] = A + (size_t)from * (WHAT == kForward ? sh.K : sh.N);
+            }
+        }
+    }
+    uint4v p_hold[kChunks], q_hold[kChunks];
+    auto fetch = [&](int r0) {
+#pragma unroll
+        for (int n = 0; n < kChunks; ++n) {
+            const int id = tid + n * kThreads;
+            if constexpr (PT) {
+                const int r = r0 + id / Elem<T>::kRowChunks;
+                long long from = -1;
+                if (r < depth) {
+                    from = r;
+                    if constexpr (WHAT == kWeights) {
+                        from = first + r;
+                        if (slot) {
+                            const int s = slot[from];
+                            from = (unsigned)s < (unsigned)sh.M ? s / sh.k : -1;
+                        }
+                    }
+                }
+                p_hold[n] = load_chunk<T, ALIGNED>(p_src[n] + (from < 0 ? 0 : from * sh.K), from < 0 ? 0 : p_valid[n]);
+            } else {
+                const int r = r0 + id % 8 * V;
+                p_hold[n] = load_chunk<T, ALIGNED>(p_src[n] + r, p_src[n] ? depth - r : 0);
+            }
+            if constexpr (QT) {
+                const int r = r0 + id / Elem<T>::kRowChunks;
+                q_hold[n] = load_chunk<T, ALIGNED>(q_src[n] + (size_t)(first + (r < depth ? r : 0)) * sh.N,
+                                                   r < depth ? q_valid[n] : 0);
+            } else {
+                const int r = r0 + id % 8 * V;
+                q_hold[n] = load_chunk<T, ALIGNED>(q_src[n] + r, q_src[n] ? depth - r : 0);
+            }
+        }
+    };
+    auto put = [&](int buffer) {
+#pragma unroll
+        for (int n = 0; n < kChunks; ++n) {
+            const int id = tid + n * kThreads;
+            const int p_at = PT ? place_turned<T>(id / Elem<T>::kRowChunks, id % Elem<T>::kRowChunks)
+                                : place_rows<T>(id / 8, id % 8);
+            const int q_at = QT ? place_turned<T>(id / Elem<T>::kRowChunks, id % Elem<T>::kRowChunks)
+                                : place_rows<T>(id / 8, id % 8);
+            *reinterpret_cast<uint4v *>(stage_p[buffer] + p_at) = p_hold[n];
+            *reinterpret_cast<uint4v *>(stage_q[buffer] + q_at) = q_hold[n];
+        }
+    };
+
+    float4v acc[4][4] = {};  // [q][p]
+    const int p_base = (wave & 1) * 64, q_base = (wave >> 1) * 64;
+    if (depth > 0) {
+        fetch(0);
+        put(0);
+    }
+    __syncthreads();
+    int buffer = 0;
+    for (int r0 = 0; r0 < depth; r0 += DEPTH) {
+        const bool more = r0 + DEPTH < depth;
+        if (more) fetch(r0 + DEPTH);
+#pragma unroll
+        for (int s = 0; s < DEPTH / Elem<T>::kStep; ++s) {
+            uint4v p[4], q[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                p[n] = fragment<T, PT>(stage_p[buffer], p_base + 16 * n, s, lane);
+                q[n] = fragment<T, QT>(stage_q[buffer], q_base + 16 * n, s, lane);
+            }
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) acc[a][b] = mma<T>(p[b], q[a], acc[a][b]);
+        }
+        if (more) put(buffer ^ 1);
+        __syncthreads();
+        buffer ^= 1;
+    }
+
+    // Lane: q = lane % 16, four p from (lane / 16) * 4 on.
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+        const int q = q_base + 16 * a + (lane & 15);
+        if (q >= rows) continue;
+        T *row = out + (WHAT == kWeights ? (size_t)expert * sh.N * sh.K + (size_t)(row0 + q) * sh.K
+                                         : (size_t)(row0 + q) * cols);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int p = col0 + p_base + 16 * b + (lane >> 4) * 4;
+            const float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
+            if (p < cols) store_vec<T, 4, ALIGNED>(row + p, v, cols - p);
+        }
+    }
+}
+
+template <typename T, Product WHAT>
+int launch_experts(const void *A, const void *B, void *out, const int *ptr, const int *slot, int k, int M, int E, int N,
+                   int K, hipStream_t st)
+{
+    ExpertsShape sh{M, E, N, K, k, 0, 0};
+    sh.col_tiles = ceil_div(WHAT == kForward ? N : K, kTile);
+    sh.row_tiles = ceil_div(N, kTile);
+    const long long others = WHAT == kWeights ? (long long)E * sh.row_tiles : num_row_tiles(M, E, kTile);
+    if (others * sh.col_tiles > INT_MAX) return MPS_ERR_UNSUPPORTED;
+    const unsigned grid = (unsigned)(others * sh.col_tiles);
+    // every operand's rows are N or K long
+    const bool fast = rows_of_16(A, WHAT == kForward ? K : N, sizeof(T)) && rows_of_16(B, K, sizeof(T)) &&
+                      rows_of_16(out, WHAT == kForward ? N : K, sizeof(T));
+#define MPS_LAUNCH_EXPERTS(ALIGNED)                                                                              \
+    hipLaunchKernelGGL((experts_tile_kernel<T, WHAT, ALIGNED>), dim3(grid), dim3(kThreads), 0, st,               \
+                       static_cast<const T *>(A), static_cast<const T *>(B), static_cast<T *>(out), ptr, slot, sh)
+    if (fast) MPS_LAUNCH_EXPERTS(true);
+    else MPS_LAUNCH_EXPERTS(false);
+#undef MPS_LAUNCH_EXPERTS
+    MPS_HIP_TRY(hipGetLastError());
+    return MPS_OK;
+}
+
+template <Product WHAT>
+int experts_entry(const void *A, const void *B, void *out, int dtype, const int *ptr, const int *slot, int k, int M,
+                  int E, int N, int K, void *stream)
+{
+    const int eb = dtype_bytes(dtype);
+    if (!eb || M < 0 || E < 1 || N < 1 || K < 1 || k < 1 || M % k) return MPS_ERR_INVALID_ARG;
+    if (M > INT_MAX - 65536 || N > INT_MAX / 4 || K > INT_MAX / 4) return MPS_ERR_UNSUPPORTED;
+    if (!ptr || (M > 0 && !A) || (M > 0 || WHAT == kWeights ? !out : false) || (M > 0 && !B)) return MPS_ERR_INVALID_ARG;
+    if (!aligned_to(A, eb) || !aligned_to(B, eb) || !aligned_to(out, eb) || !aligned_to(ptr, 4) || !aligned_to(slot, 4))
+        return MPS_ERR_ALIGNMENT;
+    if (M == 0 && WHAT != kWeights) return MPS_OK;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == MPS_F32) return launch_experts<float, WHAT>(A, B, out, ptr, slot, k, M, E, N, K, st);
+    if (dtype == MPS_F16) return launch_experts<half_t, WHAT>(A, B, out, ptr, slot, k, M, E, N, K, st);
+    return launch_experts<bf16_t, WHAT>(A, B, out, ptr, slot, k, M, E, N, K, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mps_experts_mm(const void *d_X, const void *d_W, void *d_Y, int dtype, const int *d_expert_ptr, const int *d_slot,
+                   int k, int M, int E, int N, int K, void *stream)
+{
+    return experts_entry<kForward>(d_X, d_W, d_Y, dtype, d_expert_ptr, d_slot, k, M, E, N, K, stream);
+}
+
+int mps_experts_mm_dx(const void *d_dY, const void *d_W, void *d_dX, int dtype, const int *d_expert_ptr, int M, int E,
+                      int N, int K, void *stream)
+{
+    return experts_entry<kRows>(d_dY, d_W, d_dX, dtype, d_expert_ptr, nullptr, 1, M, E, N, K, stream);
+}
+
+int mps_experts_mm_dw(const void *d_dY, const void *d_X, void *d_dW, int dtype, const int *d_expert_ptr,
+                      const int *d_slot, int k, int M, int E, int N, int K, void *stream)
+{
+    return experts_entry<kWeights>(d_dY, d_X, d_dW, dtype, d_expert_ptr, d_slot, k, M, E, N, K, stream);
+}
+
+}  // extern "C"

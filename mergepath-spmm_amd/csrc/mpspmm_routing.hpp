@@ -1,0 +1,193 @@
+// Shared by the sparse-routing translation units (mpspmm_route.hip: routing
+// matrices, their gradient, combination; mpspmm_experts.hip: the experts'
+// products; mpspmm_adapters.hip: low-rank adapters).  Everything lives in an
+// anonymous namespace.
+#ifndef MPSPMM_ROUTING_HPP
+#define MPSPMM_ROUTING_HPP
+
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cstdint>
+#include <cstring>
+
+#include "mpspmm.h"
+
+#define MPS_HIP_TRY(expr)                                       \
+    do {                                                        \
+        hipError_t e_ = (expr);                                 \
+        if (e_ != hipSuccess) return MPS_ERR_HIP + (int)e_;     \
+    } while (0)
+
+namespace {
+
+using half_t = _Float16;
+using bf16_t = __bf16;
+
+inline int dtype_bytes(int dtype) { return dtype == MPS_F32 ? 4 : (dtype == MPS_F16 || dtype == MPS_BF16) ? 2 : 0; }
+
+inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// A matrix whose rows are loaded 16 bytes at a time: aligned base, rows of whole 16 bytes.
+inline bool rows_of_16(const void *p, long long row_elems, int elem_bytes)
+{
+    return aligned_to(p, 16) && row_elems * elem_bytes % 16 == 0;
+}
+
+// V elements of T at an address that is only aligned to the element.
+template <typename T, int V>
+struct Vec {
+    typedef T type __attribute__((ext_vector_type(V)));
+};
+template <typename T>
+struct Vec<T, 1> {
+    using type = T;
+};
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void load_vec(float (&out)[V], const T *p, int valid)
+{
+    if (valid >= V) {
+        T raw[V];
+        if constexpr (ALIGNED) __builtin_memcpy(raw, __builtin_assume_aligned(p, V * sizeof(T)), V * sizeof(T));
+        else __builtin_memcpy(raw, __builtin_assume_aligned(p, sizeof(T)), V * sizeof(T));
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = (float)raw[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = i < valid ? (float)p[i] : 0.0f;
+    }
+}
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void store_vec(T *p, const float (&v)[V], int valid)
+{
+    if (valid >= V) {
+        T raw[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) raw[i] = (T)v[i];
+        if constexpr (ALIGNED) __builtin_memcpy(__builtin_assume_aligned(p, V * sizeof(T)), raw, V * sizeof(T));
+        else __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), raw, V * sizeof(T));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < valid) p[i] = (T)v[i];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Segments.  ptr[0 .. E] cuts the places 0 .. M - 1 into the experts' runs.
+// Values are clamped so that no caller's table reaches outside the arrays.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int clamp_place(int v, int M) { return min(max(v, 0), M); }
+
+// Row tiles of the segments, BM rows each.  Expert e's tiles get the numbers
+// ptr[e] / BM + e + i, i = 0 .. ceil(rows / BM) - 1.  Because
+//   floor(ptr[e] / BM) + ceil(rows / BM) <= floor(ptr[e + 1] / BM) + 1
+// no two experts share a number, so that a tile finds its expert as the last e
+// with ptr[e] / BM + e <= number, without a prefix sum over the experts: the
+// path that merges the ends of the experts with the tiles' rows.  Numbers
+// below M / BM + E; those in a gap belong to nobody (rows = 0).
+// One wavefront looks the expert up, 64 candidates at a time.
+struct RowTile {
+    int expert, first, rows;  // rows <= BM; 0 = nothing to do
+};
+template <int BM>
+__device__ __forceinline__ RowTile find_row_tile(const int *__restrict__ ptr, int E, int M, int number)
+{
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = E - 1;  // the expert lies in [lo, hi]
+    while (hi > lo) {
+        const int step = (hi - lo + 64) >> 6;
+        const int e = lo + (lane + 1) * step;
+        const bool below = e <= hi && clamp_place(ptr[e], M) / BM + e <= number;
+        const int n = __popcll(__ballot(below));
+        lo += n * step;
+        hi = min(hi, lo + step - 1);
+    }
+    const int a = clamp_place(ptr[lo], M), b = clamp_place(ptr[lo + 1], M);
+    RowTile t;
+    t.expert = lo;
+    t.first = a + (number - (a / BM + lo)) * BM;
+    t.rows = number < a / BM + lo ? 0 : min(max(b - t.first, 0), BM);
+    return t;
+}
+inline long long num_row_tiles(int M, int E, int BM) { return (long long)M / BM + E; }
+
+// ---------------------------------------------------------------------------
+// Reductions over groups of L neighbouring lanes; every lane gets the result.
+// ---------------------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v)
+{
+    return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int STEP>
+__device__ __forceinline__ unsigned lane_partner(unsigned v)
+{
+    if constexpr (STEP == 1) return dpp<0xB1>(v);         // quad_perm 1,0,3,2
+    else if constexpr (STEP == 2) return dpp<0x4E>(v);    // quad_perm 2,3,0,1
+    else if constexpr (STEP == 4) return dpp<0x141>(v);   // the other half of 8 lanes (quads agree already)
+    else if constexpr (STEP == 8) return dpp<0x140>(v);   // the other half of 16 lanes
+    else return (unsigned)__shfl_xor((int)v, STEP, 64);
+}
+template <int L>
+__device__ __forceinline__ unsigned group_max(unsigned v)
+{
+    if constexpr (L > 1) v = max(v, lane_partner<1>(v));
+    if constexpr (L > 2) v = max(v, lane_partner<2>(v));
+    if constexpr (L > 4) v = max(v, lane_partner<4>(v));
+    if constexpr (L > 8) v = max(v, lane_partner<8>(v));
+    if constexpr (L > 16) v = max(v, lane_partner<16>(v));
+    if constexpr (L > 32) v = max(v, lane_partner<32>(v));
+    return v;
+}
+template <int STEP>
+__device__ __forceinline__ unsigned long long lane_partner64(unsigned long long v)
+{
+    return ((unsigned long long)lane_partner<STEP>((unsigned)(v >> 32)) << 32) | lane_partner<STEP>((unsigned)v);
+}
+template <int L>
+__device__ __forceinline__ unsigned long long group_max(unsigned long long v)
+{
+    if constexpr (L > 1) v = max(v, lane_partner64<1>(v));
+    if constexpr (L > 2) v = max(v, lane_partner64<2>(v));
+    if constexpr (L > 4) v = max(v, lane_partner64<4>(v));
+    if constexpr (L > 8) v = max(v, lane_partner64<8>(v));
+    if constexpr (L > 16) v = max(v, lane_partner64<16>(v));
+    if constexpr (L > 32) v = max(v, lane_partner64<32>(v));
+    return v;
+}
+__device__ __forceinline__ float bits_float(unsigned u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ unsigned float_bits(float f) { return __builtin_bit_cast(unsigned, f); }
+template <int L>
+__device__ __forceinline__ float group_sum(float v)
+{
+    if constexpr (L > 1) v += bits_float(lane_partner<1>(float_bits(v)));
+    if constexpr (L > 2) v += bits_float(lane_partner<2>(float_bits(v)));
+    if constexpr (L > 4) v += bits_float(lane_partner<4>(float_bits(v)));
+    if constexpr (L > 8) v += bits_float(lane_partner<8>(float_bits(v)));
+    if constexpr (L > 16) v += bits_float(lane_partner<16>(float_bits(v)));
+    if constexpr (L > 32) v += bits_float(lane_partner<32>(float_bits(v)));
+    return v;
+}
+template <int STEP>
+__device__ __forceinline__ double lane_partner_f64(double v)
+{
+    return __builtin_bit_cast(double, lane_partner64<STEP>(__builtin_bit_cast(unsigned long long, v)));
+}
+template <int L>
+__device__ __forceinline__ double group_sum(double v)
+{
+    if constexpr (L > 1) v += lane_partner_f64<1>(v);
+    if constexpr (L > 2) v += lane_partner_f64<2>(v);
+    if constexpr (L > 4) v += lane_partner_f64<4>(v);
+    if constexpr (L > 8) v += lane_partner_f64<8>(v);
+    if constexpr (L > 16) v += lane_partner_f64<16>(v);
+    if constexpr (L > 32) v += lane_partner_f64<32>(v);
+    return v;
+}
+
+}  // namespace
+
+#endif
