@@ -73,30 +73,38 @@ __device__ __forceinline__ float4v mma(uint4v p, uint4v q, float4v acc)
     }
 }
 
-// What a lane feeds to the matrix instruction for 16 neighbouring outer
-// indices from `outer` on and matrix step s.
+// What a lane feeds to the matrix instruction for 16 neighbouring outer indices,
+// the (first + n)-th 16 of a panel, and matrix step s.  The places above differ
+// between n and s by sums and exclusive ors of constants only, so that a lane
+// needs one base: `first` a multiple of a power of two above n.
 template <typename T, bool TURNED>
-__device__ __forceinline__ uint4v fragment(const char *stage, int outer, int s, int lane)
+__device__ __forceinline__ int fragment_base(int first, int lane)
 {
     const int i = lane & 15, g = lane >> 4;
+    if constexpr (!TURNED) return place_rows<T>(first * 16 + i, g);
+    else if constexpr (sizeof(T) == 2) return place_turned<T>(8 * g + (i >> 2), first * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
+    else return place_turned<T>(4 * g, first * 4 + (i >> 2)) + (i & 3) * 4;
+}
+template <typename T, bool TURNED>
+__device__ __forceinline__ uint4v fragment(const char *panel, int base, int n, int s)
+{
     if constexpr (!TURNED) {
-        return *reinterpret_cast<const uint4v *>(stage + place_rows<T>(outer + i, 4 * s + g));
+        return *reinterpret_cast<const uint4v *>(panel + (base ^ (s << 6)) + n * 2048);
     } else if constexpr (sizeof(T) == 2) {
         // 16 lanes read a block of 4 rows (r) by 16 elements, 8 bytes each, and get it turned
-        const int row = 32 * s + 8 * g + (i >> 2), c = outer / 8 + ((i & 3) >> 1), half = (i & 1) * 8;
+        const char *at = panel + (base ^ (n << 5)) + s * 8192;
         union {
             short4v part[2];
             uint4v all;
         } u;
-        u.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)(stage + place_turned<T>(row, c) + half));
-        u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)(stage + place_turned<T>(row + 4, c) + half));
+        u.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)at);
+        u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)(at + 1024));
         return u.all;
     } else {
+        const char *at = panel + (base ^ (n << 6)) + s * 8192;
         uint4v v;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            v[j] = *reinterpret_cast<const unsigned *>(stage + place_turned<T>(16 * s + 4 * g + j, (outer + i) / 4) +
-                                                       (i & 3) * 4);
+        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const unsigned *>(at + j * 512);
         return v;
     }
 }
@@ -138,8 +146,9 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int cols = WHAT == kForward ? sh.N : sh.K;
-    const int col0 = (int)(blockIdx.x % sh.col_tiles) * kTile;
-    const int rest = blockIdx.x / sh.col_tiles;
+    const int number = xcd_tile(blockIdx.x, gridDim.x);
+    const int col0 = number % sh.col_tiles * kTile;
+    const int rest = number / sh.col_tiles;
     int expert, row0, rows, first, depth;  // rows of the tile in the result; places summed over from `first` on
     if constexpr (WHAT == kWeights) {
         expert = rest / sh.row_tiles;
@@ -236,6 +245,7 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
 
     float4v acc[4][4] = {};  // [q][p]
     const int p_base = (wave & 1) * 64, q_base = (wave >> 1) * 64;
+    const int p_at = fragment_base<T, PT>(p_base / 16, lane), q_at = fragment_base<T, QT>(q_base / 16, lane);
     if (depth > 0) {
         fetch(0);
         put(0);
@@ -250,8 +260,8 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
             uint4v p[4], q[4];
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-                p[n] = fragment<T, PT>(stage_p[buffer], p_base + 16 * n, s, lane);
-                q[n] = fragment<T, QT>(stage_q[buffer], q_base + 16 * n, s, lane);
+                p[n] = fragment<T, PT>(stage_p[buffer], p_at, n, s);
+                q[n] = fragment<T, QT>(stage_q[buffer], q_at, n, s);
             }
 #pragma unroll
             for (int a = 0; a < 4; ++a)
@@ -279,6 +289,206 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
     }
 }
 
+// The same products where rows are whole 16 bytes.  The stages come straight
+// from memory into LDS, two of them in turn: while the matrix instructions work
+// on one, the other is on its way.  A chunk that does not exist (rows behind
+// the segment, columns behind the matrix, the end of the sum) is taken from a
+// page of zeros, so that the loop itself asks for nothing.
+//   PP, QP  panels of 128 in the tile's columns and rows
+//   WP, WQ  wavefronts that share them
+__device__ const uint4v zero_page[1] = {{0, 0, 0, 0}};
+
+typedef const __attribute__((address_space(1))) void *global_ptr;
+typedef __attribute__((address_space(3))) void *lds_ptr;
+
+template <typename T, Product WHAT, int PP, int QP, int WP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T *__restrict__ A, const T *__restrict__ B,
+                                                                         T *__restrict__ out,
+                                                                         const int *__restrict__ ptr,
+                                                                         const int *__restrict__ slot, ExpertsShape sh)
+{
+    constexpr bool PT = WHAT != kForward, QT = WHAT == kWeights;
+    constexpr int V = Elem<T>::kPerChunk, DEPTH = Elem<T>::kDepth, ROW = Elem<T>::kRowChunks;
+    constexpr int THREADS = 64 * WP * WQ, BP = PP * kTile, BQ = QP * kTile, PANEL = kTile * 128;
+    constexpr int PC = PP * PANEL / 16 / THREADS, QC = QP * PANEL / 16 / THREADS;  // chunks of a thread
+    constexpr int FP = BP / 16 / WP, FQ = BQ / 16 / WQ;                           // fragments of a wavefront
+    __shared__ __attribute__((aligned(16))) char stage0[(PP + QP) * PANEL];
+    __shared__ __attribute__((aligned(16))) char stage1[(PP + QP) * PANEL];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int cols = WHAT == kForward ? sh.N : sh.K;
+    const int number = xcd_tile(blockIdx.x, gridDim.x);
+    const int col0 = number % sh.col_tiles * BP;
+    const int rest = number / sh.col_tiles;
+    int expert, row0, rows, first, depth;
+    if constexpr (WHAT == kWeights) {
+        expert = rest / sh.row_tiles;
+        row0 = rest % sh.row_tiles * BQ;
+        rows = min(sh.N - row0, BQ);
+        first = clamp_place(ptr[expert], sh.M);
+        depth = max(clamp_place(ptr[expert + 1], sh.M) - first, 0);
+    } else {
+        const RowTile t = find_row_tile<BQ>(ptr, sh.E, sh.M, rest);
+        if (t.rows == 0) return;
+        expert = t.expert;
+        row0 = first = t.first;
+        rows = t.rows;
+        depth = WHAT == kForward ? sh.K : sh.N;
+    }
+    const T *W = WHAT == kWeights ? nullptr : B + (size_t)expert * sh.N * sh.K;
+    const T *const zeros = reinterpret_cast<const T *>(zero_page);
+
+    // Chunk n of this thread lies at (n * THREADS + tid) * 16 of its operand.
+    // Kept for each: where it comes from next, and the summed index it begins with
+    // in a stage; kNever for one that holds zeros throughout.
+    constexpr int kNever = 1 << 30;
+    const T *p_src[PC], *q_src[QC];
+    int p_r[PC], q_r[QC];
+    const long long p_step = PT ? (long long)DEPTH * sh.K : DEPTH, q_step = QT ? (long long)DEPTH * sh.N : DEPTH;
+    constexpr bool LIST = WHAT == kWeights;  // rows of P are looked up for every stage
+#pragma unroll
+    for (int n = 0; n < PC; ++n) {
+        const int id = n * THREADS + tid, panel = id / (PANEL / 16), in = id % (PANEL / 16);
+        if constexpr (PT) {
+            const int row = in / ROW, c = place_turned<T>(row, in % ROW) / 16 % ROW;
+            const int col = col0 + panel * kTile + c * V;
+            p_r[n] = col < cols ? row : kNever;
+            p_src[n] = (LIST ? B : W + (size_t)row * sh.K) + col;
+        } else {
+            const int row = in / 8, c = place_rows<T>(row, in % 8) / 16 % 8;
+            const int col = col0 + panel * kTile + row;
+            p_r[n] = col < cols ? c * V : kNever;
+            p_src[n] = W + (size_t)col * sh.K + c * V;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < QC; ++n) {
+        const int id = n * THREADS + tid, panel = id / (PANEL / 16), in = id % (PANEL / 16);
+        if constexpr (QT) {
+            const int row = in / ROW, c = place_turned<T>(row, in % ROW) / 16 % ROW;
+            const int at = row0 + panel * kTile + c * V;
+            q_r[n] = at < sh.N ? row : kNever;
+            q_src[n] = A + (size_t)(first + row) * sh.N + at;
+        } else {
+            const int row = in / 8, c = place_rows<T>(row, in % 8) / 16 % 8;
+            const int at = panel * kTile + row;
+            int from = at < rows ? first + at : -1;
+            if (WHAT == kForward && slot && from >= 0) {
+                const int s = slot[from];
+                from = (unsigned)s < (unsigned)sh.M ? s / sh.k : -1;
+            }
+            q_r[n] = from >= 0 ? c * V : kNever;
+            q_src[n] = A + (long long)from * (WHAT == kForward ? sh.K : sh.N) + c * V;
+        }
+    }
+    // Rows of P for the next stage (dW): looked up one stage ahead.
+    int row_of[PC];
+    auto look_up = [&](int r0) {
+#pragma unroll
+        for (int n = 0; n < PC; ++n) {
+            const int r = r0 + p_r[n];
+            int from = r < depth ? first + r : -1;
+            if (slot && from >= 0) from = slot[from];
+            row_of[n] = from;
+        }
+    };
+    auto issue = [&](char *stage, int r0) {
+#pragma unroll
+        for (int n = 0; n < PC; ++n) {
+            const T *from;
+            if constexpr (LIST) {
+                const int s = row_of[n];
+                const bool is = slot ? (unsigned)s < (unsigned)sh.M : s >= 0;
+                from = is ? p_src[n] + (long long)(slot ? s / sh.k : s) * sh.K : zeros;
+            } else {
+                from = r0 + p_r[n] < depth ? p_src[n] : zeros;
+                p_src[n] += p_step;
+            }
+            __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)(stage + (n * THREADS + wave * 64) * 16), 16, 0, 0);
+        }
+#pragma unroll
+        for (int n = 0; n < QC; ++n) {
+            const T *from = r0 + q_r[n] < depth ? q_src[n] : zeros;
+            q_src[n] += q_step;
+            __builtin_amdgcn_global_load_lds((global_ptr)from,
+                                             (lds_ptr)(stage + PP * PANEL + (n * THREADS + wave * 64) * 16), 16, 0, 0);
+        }
+    };
+
+    float4v acc[FQ][FP] = {};
+    const int p_base = wave % WP * (FP * 16), q_base = wave / WP * (FQ * 16);
+    static_assert(FP <= 8 && FQ <= 8, "a wavefront's part of an operand lies in one panel");
+    const int p_at = p_base / kTile * PANEL + fragment_base<T, PT>(p_base % kTile / 16, lane);
+    const int q_at = (PP + q_base / kTile) * PANEL + fragment_base<T, QT>(q_base % kTile / 16, lane);
+    auto work = [&](const char *stage) {
+#pragma unroll
+        for (int s = 0; s < DEPTH / Elem<T>::kStep; ++s) {
+            uint4v p[FP], q[FQ];
+            // fragments of one step at a time: those of two, and the sums, are more than the registers
+            if (FP * FQ > 16) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int n = 0; n < FP; ++n) p[n] = fragment<T, PT>(stage, p_at, n, s);
+#pragma unroll
+            for (int n = 0; n < FQ; ++n) q[n] = fragment<T, QT>(stage, q_at, n, s);
+#pragma unroll
+            for (int a = 0; a < FQ; ++a)
+#pragma unroll
+                for (int b = 0; b < FP; ++b) acc[a][b] = mma<T>(p[b], q[a], acc[a][b]);
+        }
+    };
+    auto arrive = [] {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): own chunks have come, own reads of LDS are done
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    // Two stages a turn, behind the end of the sum ones of zeros.
+    if constexpr (LIST) look_up(0);
+    issue(stage0, 0);
+    if constexpr (LIST) look_up(DEPTH);
+    for (int r0 = 0; r0 < depth; r0 += 2 * DEPTH) {
+        arrive();  // stage 0 has come, and everybody is done with stage 1
+        issue(stage1, r0 + DEPTH);
+        if constexpr (LIST) look_up(r0 + 2 * DEPTH);
+        work(stage0);
+        arrive();
+        issue(stage0, r0 + 2 * DEPTH);
+        if constexpr (LIST) look_up(r0 + 3 * DEPTH);
+        work(stage1);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070);  // nothing is on its way into LDS when the workgroup ends
+
+#pragma unroll
+    for (int a = 0; a < FQ; ++a) {
+        const int q = q_base + 16 * a + (lane & 15);
+        if (q >= rows) continue;
+        T *row = out + (WHAT == kWeights ? (size_t)expert * sh.N * sh.K + (size_t)(row0 + q) * sh.K
+                                         : (size_t)(row0 + q) * cols);
+#pragma unroll
+        for (int b = 0; b < FP; ++b) {
+            const int p = col0 + p_base + 16 * b + (lane >> 4) * 4;
+            const float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
+            if (p < cols) store_vec<T, 4, true>(row + p, v, cols - p);
+        }
+    }
+}
+
+template <typename T, Product WHAT, int PP, int QP, int WP, int WQ>
+int launch_stream(const void *A, const void *B, void *out, const int *ptr, const int *slot, ExpertsShape sh, hipStream_t st)
+{
+    sh.col_tiles = ceil_div(WHAT == kForward ? sh.N : sh.K, PP * kTile);
+    sh.row_tiles = ceil_div(sh.N, QP * kTile);
+    const long long others = WHAT == kWeights ? (long long)sh.E * sh.row_tiles : num_row_tiles(sh.M, sh.E, QP * kTile);
+    if (others * sh.col_tiles > INT_MAX) return MPS_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((experts_stream_kernel<T, WHAT, PP, QP, WP, WQ>), dim3((unsigned)(others * sh.col_tiles)),
+                       dim3(64 * WP * WQ), 0, st, static_cast<const T *>(A), static_cast<const T *>(B),
+                       static_cast<T *>(out), ptr, slot, sh);
+    MPS_HIP_TRY(hipGetLastError());
+    return MPS_OK;
+}
+
 template <typename T, Product WHAT>
 int launch_experts(const void *A, const void *B, void *out, const int *ptr, const int *slot, int k, int M, int E, int N,
                    int K, hipStream_t st)
@@ -292,11 +502,15 @@ int launch_experts(const void *A, const void *B, void *out, const int *ptr, cons
     // every operand's rows are N or K long
     const bool fast = rows_of_16(A, WHAT == kForward ? K : N, sizeof(T)) && rows_of_16(B, K, sizeof(T)) &&
                       rows_of_16(out, WHAT == kForward ? N : K, sizeof(T));
+    if (fast) {
+        if (sizeof(T) == 2 && (long long)M >= 384LL * E)
+            return launch_stream<T, WHAT, 2, 2, 2, 4>(A, B, out, ptr, slot, sh, st);
+        return launch_stream<T, WHAT, 1, 1, 2, 2>(A, B, out, ptr, slot, sh, st);
+    }
 #define MPS_LAUNCH_EXPERTS(ALIGNED)                                                                              \
     hipLaunchKernelGGL((experts_tile_kernel<T, WHAT, ALIGNED>), dim3(grid), dim3(kThreads), 0, st,               \
                        static_cast<const T *>(A), static_cast<const T *>(B), static_cast<T *>(out), ptr, slot, sh)
-    if (fast) MPS_LAUNCH_EXPERTS(true);
-    else MPS_LAUNCH_EXPERTS(false);
+    MPS_LAUNCH_EXPERTS(false);
 #undef MPS_LAUNCH_EXPERTS
     MPS_HIP_TRY(hipGetLastError());
     return MPS_OK;

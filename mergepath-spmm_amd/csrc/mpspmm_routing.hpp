@@ -112,6 +112,17 @@ __device__ __forceinline__ RowTile find_row_tile(const int *__restrict__ ptr, in
     t.rows = number < a / BM + lo ? 0 : min(max(b - t.first, 0), BM);
     return t;
 }
+// Workgroups are dealt to the 8 dies in turn, each with an L2 of its own.  Runs
+// of kRun tiles go to one die, as many as it works on at a time, so that the
+// tiles that share an expert's weights and rows meet in one L2; the runs are
+// dealt in turn, so that a long segment is shared by all dies.
+__device__ __forceinline__ int xcd_tile(int block, int blocks)
+{
+    constexpr int kRun = 64;
+    if (block >= blocks / (8 * kRun) * (8 * kRun)) return block;
+    const int xcd = block & 7, nth = block >> 3;
+    return ((nth / kRun) * 8 + xcd) * kRun + nth % kRun;
+}
 inline long long num_row_tiles(int M, int E, int BM) { return (long long)M / BM + E; }
 
 // ---------------------------------------------------------------------------
