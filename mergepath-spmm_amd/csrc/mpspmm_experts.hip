@@ -291,14 +291,9 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
 
 // The same products where rows are whole 16 bytes.  The stages come straight
 // from memory into LDS, two of them in turn: while the matrix instructions work
-// on one, the other is on its way.  A chunk that does not exist (rows behind
-// the segment, columns behind the matrix, the end of the sum) is taken from a
-// page of zeros, so that the loop itself asks for nothing.
+// on one, the other is on its way.
 //   PP, QP  panels of 128 in the tile's columns and rows
 //   WP, WQ  wavefronts that share them
-__device__ const uint4v zero_page[1] = {{0, 0, 0, 0}};
-
-typedef const __attribute__((address_space(1))) void *global_ptr;
 typedef __attribute__((address_space(3))) void *lds_ptr;
 
 template <typename T, Product WHAT, int PP, int QP, int WP, int WQ>
@@ -331,89 +326,99 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     } else {
         const RowTile t = find_row_tile<BQ>(ptr, sh.E, sh.M, rest);
         if (t.rows == 0) return;
-        expert = t.expert;
-        row0 = first = t.first;
-        rows = t.rows;
+        expert = __builtin_amdgcn_readfirstlane(t.expert);
+        row0 = first = __builtin_amdgcn_readfirstlane(t.first);
+        rows = __builtin_amdgcn_readfirstlane(t.rows);
         depth = WHAT == kForward ? sh.K : sh.N;
     }
-    const T *W = WHAT == kWeights ? nullptr : B + (size_t)expert * sh.N * sh.K;
-    const T *const zeros = reinterpret_cast<const T *>(zero_page);
 
-    // Chunk n of this thread lies at (n * THREADS + tid) * 16 of its operand.
-    // Kept for each: where it comes from next, and the summed index it begins with
-    // in a stage; kNever for one that holds zeros throughout.
-    constexpr int kNever = 1 << 30;
-    const T *p_src[PC], *q_src[QC];
-    int p_r[PC], q_r[QC];
-    const long long p_step = PT ? (long long)DEPTH * sh.K : DEPTH, q_step = QT ? (long long)DEPTH * sh.N : DEPTH;
+    // Chunk n of this thread lies at (n * THREADS + tid) * 16 of its operand.  It
+    // comes from the stage's base, which all threads share, plus an offset of 32
+    // bits (the launcher sees to that).  A row or column that does not exist is
+    // replaced by the last one that does: what is made of it is not stored.
+    // Chunks behind the end of the sum, and rows whose slot is out of range, are
+    // asked for behind the end of the buffer, which gives zeros.
+    constexpr unsigned kBufferEnd = 0x80000000u;
+    const char *p_now, *q_now;
+    unsigned p_off[PC], q_off[QC];
+    const long long p_step = (PT ? (long long)DEPTH * sh.K : DEPTH) * (long long)sizeof(T);
+    const long long q_step = (QT ? (long long)DEPTH * sh.N : DEPTH) * (long long)sizeof(T);
     constexpr bool LIST = WHAT == kWeights;  // rows of P are looked up for every stage
+    // where chunk n begins in its staged row, and the summed index it begins with in a stage
+    auto turned_at = [&](int n) { return place_turned<T>(tid / ROW + n * THREADS / ROW % DEPTH, tid % ROW) / 16 % ROW * V; };
+    const int row_at = place_rows<T>(tid / 8, tid % 8) / 16 % 8 * V;  // the same for all n
+    static_assert(THREADS / 8 % 16 == 0, "rows of equal place");
+    auto p_r = [&](int n) { return PT ? tid / ROW + n * THREADS / ROW % DEPTH : row_at; };
+    auto q_r = [&](int n) { return QT ? tid / ROW + n * THREADS / ROW % DEPTH : row_at; };
 #pragma unroll
     for (int n = 0; n < PC; ++n) {
-        const int id = n * THREADS + tid, panel = id / (PANEL / 16), in = id % (PANEL / 16);
+        const int panel = n * THREADS / (PANEL / 16);
         if constexpr (PT) {
-            const int row = in / ROW, c = place_turned<T>(row, in % ROW) / 16 % ROW;
-            const int col = col0 + panel * kTile + c * V;
-            p_r[n] = col < cols ? row : kNever;
-            p_src[n] = (LIST ? B : W + (size_t)row * sh.K) + col;
+            const int col = min(col0 + panel * kTile + turned_at(n), cols - V);
+            p_off[n] = (unsigned)((LIST ? 0u : (unsigned)p_r(n) * (unsigned)sh.K) + col) * (unsigned)sizeof(T);
         } else {
-            const int row = in / 8, c = place_rows<T>(row, in % 8) / 16 % 8;
-            const int col = col0 + panel * kTile + row;
-            p_r[n] = col < cols ? c * V : kNever;
-            p_src[n] = W + (size_t)col * sh.K + c * V;
+            const int col = min(col0 + (n * THREADS + tid) / 8, cols - 1);
+            p_off[n] = ((unsigned)col * (unsigned)sh.K + row_at) * (unsigned)sizeof(T);
         }
     }
+    p_now = reinterpret_cast<const char *>(LIST ? B : B + (size_t)expert * sh.N * sh.K);
 #pragma unroll
     for (int n = 0; n < QC; ++n) {
-        const int id = n * THREADS + tid, panel = id / (PANEL / 16), in = id % (PANEL / 16);
+        const int panel = n * THREADS / (PANEL / 16);
         if constexpr (QT) {
-            const int row = in / ROW, c = place_turned<T>(row, in % ROW) / 16 % ROW;
-            const int at = row0 + panel * kTile + c * V;
-            q_r[n] = at < sh.N ? row : kNever;
-            q_src[n] = A + (size_t)(first + row) * sh.N + at;
+            const int at = min(row0 + panel * kTile + turned_at(n), sh.N - V);
+            q_off[n] = ((unsigned)q_r(n) * (unsigned)sh.N + at) * (unsigned)sizeof(T);
         } else {
-            const int row = in / 8, c = place_rows<T>(row, in % 8) / 16 % 8;
-            const int at = panel * kTile + row;
-            int from = at < rows ? first + at : -1;
-            if (WHAT == kForward && slot && from >= 0) {
-                const int s = slot[from];
-                from = (unsigned)s < (unsigned)sh.M ? s / sh.k : -1;
+            const int at = min((n * THREADS + tid) / 8, rows - 1);
+            int from = at;
+            if constexpr (WHAT == kForward) {
+                from += first;
+                if (slot) {
+                    const int s = slot[from];
+                    const bool is = (unsigned)s < (unsigned)sh.M;
+                    from = is ? s / sh.k : -1;
+                }
             }
-            q_r[n] = from >= 0 ? c * V : kNever;
-            q_src[n] = A + (long long)from * (WHAT == kForward ? sh.K : sh.N) + c * V;
+            q_off[n] = from < 0 ? kBufferEnd
+                                : ((unsigned)from * (unsigned)(WHAT == kForward ? sh.K : sh.N) + row_at) * (unsigned)sizeof(T);
         }
     }
+    q_now = reinterpret_cast<const char *>(WHAT == kForward ? A : A + (size_t)first * sh.N);
     // Rows of P for the next stage (dW): looked up one stage ahead.
     int row_of[PC];
     auto look_up = [&](int r0) {
 #pragma unroll
         for (int n = 0; n < PC; ++n) {
-            const int r = r0 + p_r[n];
+            const int r = r0 + p_r(n);
             int from = r < depth ? first + r : -1;
             if (slot && from >= 0) from = slot[from];
             row_of[n] = from;
         }
     };
+    auto request = [&](const char *base, unsigned off, char *stage, int n) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, kBufferEnd, 0x00020000),
+            (lds_ptr)(stage + (n * THREADS + wave * 64) * 16), 16, off, 0, 0, 0);
+    };
     auto issue = [&](char *stage, int r0) {
 #pragma unroll
         for (int n = 0; n < PC; ++n) {
-            const T *from;
+            unsigned off;
             if constexpr (LIST) {
                 const int s = row_of[n];
                 const bool is = slot ? (unsigned)s < (unsigned)sh.M : s >= 0;
-                from = is ? p_src[n] + (long long)(slot ? s / sh.k : s) * sh.K : zeros;
+                const unsigned row = slot ? (unsigned)s / (unsigned)sh.k : (unsigned)s;
+                off = is ? p_off[n] + row * (unsigned)sh.K * (unsigned)sizeof(T) : kBufferEnd;
             } else {
-                from = r0 + p_r[n] < depth ? p_src[n] : zeros;
-                p_src[n] += p_step;
+                off = r0 + p_r(n) < depth ? p_off[n] : kBufferEnd;
             }
-            __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)(stage + (n * THREADS + wave * 64) * 16), 16, 0, 0);
+            request(p_now, off, stage, n);
         }
 #pragma unroll
-        for (int n = 0; n < QC; ++n) {
-            const T *from = r0 + q_r[n] < depth ? q_src[n] : zeros;
-            q_src[n] += q_step;
-            __builtin_amdgcn_global_load_lds((global_ptr)from,
-                                             (lds_ptr)(stage + PP * PANEL + (n * THREADS + wave * 64) * 16), 16, 0, 0);
-        }
+        for (int n = 0; n < QC; ++n)
+            request(q_now, r0 + q_r(n) < depth ? q_off[n] : kBufferEnd, stage + PP * PANEL, n);
+        if constexpr (!LIST) p_now += p_step;
+        q_now += q_step;
     };
 
     float4v acc[FQ][FP] = {};
@@ -421,42 +426,65 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     static_assert(FP <= 8 && FQ <= 8, "a wavefront's part of an operand lies in one panel");
     const int p_at = p_base / kTile * PANEL + fragment_base<T, PT>(p_base % kTile / 16, lane);
     const int q_at = (PP + q_base / kTile) * PANEL + fragment_base<T, QT>(q_base % kTile / 16, lane);
-    auto work = [&](const char *stage) {
-#pragma unroll
-        for (int s = 0; s < DEPTH / Elem<T>::kStep; ++s) {
-            uint4v p[FP], q[FQ];
-            // fragments of one step at a time: those of two, and the sums, are more than the registers
-            if (FP * FQ > 16) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int n = 0; n < FP; ++n) p[n] = fragment<T, PT>(stage, p_at, n, s);
-#pragma unroll
-            for (int n = 0; n < FQ; ++n) q[n] = fragment<T, QT>(stage, q_at, n, s);
-#pragma unroll
-            for (int a = 0; a < FQ; ++a)
-#pragma unroll
-                for (int b = 0; b < FP; ++b) acc[a][b] = mma<T>(p[b], q[a], acc[a][b]);
-        }
-    };
     auto arrive = [] {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): own chunks have come, own reads of LDS are done
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
+    // A stage is two matrix steps, a step two halves of P: four groups of matrix
+    // instructions.  What a group needs is read from LDS while the group before
+    // it works, across the stages too: everybody has read all of a stage before
+    // its last group, which the first reads of the next stage and the requests
+    // for the one after that go along with.
+    static_assert(DEPTH == 2 * Elem<T>::kStep, "a stage is two matrix steps");
+    constexpr int HALF = FP / 2;
+    uint4v q[2][FQ], p[2][HALF];
+    auto read_q = [&](const char *stage, int s, int to) {
+#pragma unroll
+        for (int n = 0; n < FQ; ++n) q[to][n] = fragment<T, QT>(stage, q_at, n, s);
+    };
+    auto read_p = [&](const char *stage, int s, int half) {
+#pragma unroll
+        for (int n = 0; n < HALF; ++n) p[half][n] = fragment<T, PT>(stage, p_at, half * HALF + n, s);
+    };
+    auto group = [&](int of, int half) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int a = 0; a < FQ; ++a)
+#pragma unroll
+            for (int b = 0; b < HALF; ++b) acc[a][half * HALF + b] = mma<T>(p[half][b], q[of][a], acc[a][half * HALF + b]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto turn = [&](char *now, const char *next, int r0) {
+        read_p(now, 0, 1);
+        group(0, 0);
+        read_q(now, 1, 1);
+        read_p(now, 1, 0);
+        group(0, 1);
+        read_p(now, 1, 1);
+        group(1, 0);
+        arrive();  // the next stage has come, and everybody is done with this one
+        read_q(next, 0, 0);
+        read_p(next, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        issue(now, r0 + 2 * DEPTH);
+        if constexpr (LIST) look_up(r0 + 3 * DEPTH);
+        group(1, 1);
+    };
 
     // Two stages a turn, behind the end of the sum ones of zeros.
     if constexpr (LIST) look_up(0);
     issue(stage0, 0);
     if constexpr (LIST) look_up(DEPTH);
+    arrive();
+    issue(stage1, DEPTH);
+    if constexpr (LIST) look_up(2 * DEPTH);
+    read_q(stage0, 0, 0);
+    read_p(stage0, 0, 0);
     for (int r0 = 0; r0 < depth; r0 += 2 * DEPTH) {
-        arrive();  // stage 0 has come, and everybody is done with stage 1
-        issue(stage1, r0 + DEPTH);
-        if constexpr (LIST) look_up(r0 + 2 * DEPTH);
-        work(stage0);
-        arrive();
-        issue(stage0, r0 + 2 * DEPTH);
-        if constexpr (LIST) look_up(r0 + 3 * DEPTH);
-        work(stage1);
+        turn(stage0, stage1, r0);
+        turn(stage1, stage0, r0 + DEPTH);
     }
     __builtin_amdgcn_s_waitcnt(0x0070);  // nothing is on its way into LDS when the workgroup ends
 
@@ -502,15 +530,21 @@ int launch_experts(const void *A, const void *B, void *out, const int *ptr, cons
     // every operand's rows are N or K long
     const bool fast = rows_of_16(A, WHAT == kForward ? K : N, sizeof(T)) && rows_of_16(B, K, sizeof(T)) &&
                       rows_of_16(out, WHAT == kForward ? N : K, sizeof(T));
-    if (fast) {
-        if (sizeof(T) == 2 && (long long)M >= 384LL * E)
-            return launch_stream<T, WHAT, 2, 2, 2, 4>(A, B, out, ptr, slot, sh, st);
+    // offsets of 32 bits inside X or dY and inside the matrix of an expert
+    const long long far = INT_MAX / (long long)sizeof(T);
+    const bool near = (long long)M * (WHAT == kForward ? K : N) <= far && (long long)N * K <= far &&
+                      (WHAT != kWeights || (long long)M * K <= far);
+    if (fast && near) {
+        if constexpr (sizeof(T) == 2 && WHAT != kWeights) {
+            if ((long long)M >= 384LL * E) return launch_stream<T, WHAT, 2, 2, 2, 4>(A, B, out, ptr, slot, sh, st);
+        }
         return launch_stream<T, WHAT, 1, 1, 2, 2>(A, B, out, ptr, slot, sh, st);
     }
 #define MPS_LAUNCH_EXPERTS(ALIGNED)                                                                              \
     hipLaunchKernelGGL((experts_tile_kernel<T, WHAT, ALIGNED>), dim3(grid), dim3(kThreads), 0, st,               \
                        static_cast<const T *>(A), static_cast<const T *>(B), static_cast<T *>(out), ptr, slot, sh)
-    MPS_LAUNCH_EXPERTS(false);
+    if (fast) MPS_LAUNCH_EXPERTS(true);
+    else MPS_LAUNCH_EXPERTS(false);
 #undef MPS_LAUNCH_EXPERTS
     MPS_HIP_TRY(hipGetLastError());
     return MPS_OK;
