@@ -16,6 +16,8 @@
 // four neighbouring p of one q: stores of 8 or 16 bytes.
 #include "mpspmm_routing.hpp"
 
+#include <type_traits>
+
 namespace {
 
 typedef float float4v __attribute__((ext_vector_type(4)));
@@ -129,7 +131,22 @@ __device__ __forceinline__ uint4v load_chunk(const T *p, int valid)
 struct ExpertsShape {
     int M, E, N, K, k;
     int col_tiles, row_tiles;
+    unsigned k_magic, k_shift;  // slot / k = slot * k_magic >> k_shift, see divide_by()
 };
+
+// s / k for 0 <= s < 2^31: with 2^(L - 1) < k <= 2^L and m = ceil(2^(31 + L) / k), m k exceeds 2^(31 + L) by less than
+// k <= 2^L, so that s m / 2^(31 + L) exceeds s / k by less than 1 / k.  m < 2^32.
+void divide_by(int k, unsigned &magic, unsigned &shift)
+{
+    unsigned L = 0;
+    while ((1ll << L) < k) ++L;
+    shift = 31 + L;
+    magic = (unsigned)(((1ull << shift) + (unsigned)k - 1) / (unsigned)k);
+}
+__device__ __forceinline__ unsigned token_of(unsigned slot, const ExpertsShape &sh)
+{
+    return (unsigned)(((unsigned long long)slot * sh.k_magic) >> sh.k_shift);
+}
 
 enum Product { kForward, kRows, kWeights };
 
@@ -191,7 +208,7 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
                 int from = first + row;
                 if (WHAT == kForward && slot) {
                     const int s = slot[from];
-                    from = (unsigned)s < (unsigned)sh.M ? s / sh.k : -1;
+                    from = (unsigned)s < (unsigned)sh.M ? (int)token_of(s, sh) : -1;
                 }
                 if (from >= 0) q_src[n] = A + (size_t)from * (WHAT == kForward ? sh.K : sh.N);
             }
@@ -211,7 +228,7 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
                         from = first + r;
                         if (slot) {
                             const int s = slot[from];
-                            from = (unsigned)s < (unsigned)sh.M ? s / sh.k : -1;
+                            from = (unsigned)s < (unsigned)sh.M ? (int)token_of(s, sh) : -1;
                         }
                     }
                 }
@@ -376,7 +393,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
                 if (slot) {
                     const int s = slot[from];
                     const bool is = (unsigned)s < (unsigned)sh.M;
-                    from = is ? s / sh.k : -1;
+                    from = is ? (int)token_of(s, sh) : -1;
                 }
             }
             q_off[n] = from < 0 ? kBufferEnd
@@ -407,7 +424,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
             if constexpr (LIST) {
                 const int s = row_of[n];
                 const bool is = slot ? (unsigned)s < (unsigned)sh.M : s >= 0;
-                const unsigned row = slot ? (unsigned)s / (unsigned)sh.k : (unsigned)s;
+                const unsigned row = slot ? token_of(s, sh) : (unsigned)s;
                 off = is ? p_off[n] + row * (unsigned)sh.K * (unsigned)sizeof(T) : kBufferEnd;
             } else {
                 off = r0 + p_r(n) < depth ? p_off[n] : kBufferEnd;
@@ -422,7 +439,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     };
 
     float4v acc[FQ][FP] = {};
-    const int p_base = wave % WP * (FP * 16), q_base = wave / WP * (FQ * 16);
+    // Wavefronts w and w + 4 share a SIMD.  Where there are 8 they take opposite
+    // halves of both the columns and the rows, and one whose rows or columns do not
+    // exist has no work: a tile that is half empty takes half the time.
+    constexpr bool EIGHT = WP == 2 && WQ == 4;
+    const int p_part = EIGHT ? (wave & 1) ^ (wave >> 2) : wave % WP;
+    const int q_part = EIGHT ? (wave >> 1 & 1) | (wave >> 2) << 1 : wave / WP;
+    const int p_base = p_part * (FP * 16), q_base = q_part * (FQ * 16);
+    const bool busy = q_base < rows && col0 + p_base < cols;
     static_assert(FP <= 8 && FQ <= 8, "a wavefront's part of an operand lies in one panel");
     const int p_at = p_base / kTile * PANEL + fragment_base<T, PT>(p_base % kTile / 16, lane);
     const int q_at = (PP + q_base / kTile) * PANEL + fragment_base<T, QT>(q_base % kTile / 16, lane);
@@ -456,21 +480,26 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
             for (int b = 0; b < HALF; ++b) acc[a][half * HALF + b] = mma<T>(p[half][b], q[of][a], acc[a][half * HALF + b]);
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto turn = [&](char *now, const char *next, int r0) {
-        read_p(now, 0, 1);
-        group(0, 0);
-        read_q(now, 1, 1);
-        read_p(now, 1, 0);
-        group(0, 1);
-        read_p(now, 1, 1);
-        group(1, 0);
+    auto turn = [&](auto works, char *now, const char *next, int r0) {
+        constexpr bool busy = decltype(works)::value;
+        if constexpr (busy) {
+            read_p(now, 0, 1);
+            group(0, 0);
+            read_q(now, 1, 1);
+            read_p(now, 1, 0);
+            group(0, 1);
+            read_p(now, 1, 1);
+            group(1, 0);
+        }
         arrive();  // the next stage has come, and everybody is done with this one
-        read_q(next, 0, 0);
-        read_p(next, 0, 0);
+        if constexpr (busy) {
+            read_q(next, 0, 0);
+            read_p(next, 0, 0);
+        }
         __builtin_amdgcn_sched_barrier(0);
         issue(now, r0 + 2 * DEPTH);
         if constexpr (LIST) look_up(r0 + 3 * DEPTH);
-        group(1, 1);
+        if constexpr (busy) group(1, 1);
     };
 
     // Two stages a turn, behind the end of the sum ones of zeros.
@@ -480,11 +509,18 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     arrive();
     issue(stage1, DEPTH);
     if constexpr (LIST) look_up(2 * DEPTH);
-    read_q(stage0, 0, 0);
-    read_p(stage0, 0, 0);
-    for (int r0 = 0; r0 < depth; r0 += 2 * DEPTH) {
-        turn(stage0, stage1, r0);
-        turn(stage1, stage0, r0 + DEPTH);
+    if (busy) {
+        read_q(stage0, 0, 0);
+        read_p(stage0, 0, 0);
+        for (int r0 = 0; r0 < depth; r0 += 2 * DEPTH) {
+            turn(std::true_type{}, stage0, stage1, r0);
+            turn(std::true_type{}, stage1, stage0, r0 + DEPTH);
+        }
+    } else {  // the same requests and barriers
+        for (int r0 = 0; r0 < depth; r0 += 2 * DEPTH) {
+            turn(std::false_type{}, stage0, stage1, r0);
+            turn(std::false_type{}, stage1, stage0, r0 + DEPTH);
+        }
     }
     __builtin_amdgcn_s_waitcnt(0x0070);  // nothing is on its way into LDS when the workgroup ends
 
@@ -521,7 +557,8 @@ template <typename T, Product WHAT>
 int launch_experts(const void *A, const void *B, void *out, const int *ptr, const int *slot, int k, int M, int E, int N,
                    int K, hipStream_t st)
 {
-    ExpertsShape sh{M, E, N, K, k, 0, 0};
+    ExpertsShape sh{M, E, N, K, k, 0, 0, 0, 0};
+    divide_by(k, sh.k_magic, sh.k_shift);
     sh.col_tiles = ceil_div(WHAT == kForward ? N : K, kTile);
     sh.row_tiles = ceil_div(N, kTile);
     const long long others = WHAT == kWeights ? (long long)E * sh.row_tiles : num_row_tiles(M, E, kTile);
