@@ -17,7 +17,6 @@ typedef bf16_t bf16x8v __attribute__((ext_vector_type(8)));
 typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
-constexpr int kRows = 16;  // tokens of a tile
 
 template <typename T>
 __device__ __forceinline__ float4v mma(uint4v p, uint4v q, float4v acc)
@@ -55,158 +54,204 @@ __device__ __forceinline__ uint4v load_chunk(const T *p, int valid)
 
 struct AdaptersShape {
     int T, E, R, K, N;
-    int padded;       // the rank that the kernels are made for, 16, 32, 64, 128 or 256: the pitch of V
+    int padded;             // the rank that the kernels are made for, 16, 32, 64, 128 or 256: the pitch of V
     int splits, per_split;  // parts of the sum over K, and their length
+    bool tall;              // long segments: tiles of several times 16 tokens
 };
 
 // V[split][place][r] = sum over the split's part of K.  One workgroup per tile
-// of 16 tokens and part; its four wavefronts take the 64-byte steps of the part
-// in turn and add up through LDS.
-template <typename T, int RT, bool ALIGNED>
+// of 16 MT tokens and part; its four wavefronts take 128 bytes of a row in turn
+// and add up through LDS.  A step of 64 bytes loads MT + RT chunks for MT * RT
+// matrix instructions.
+template <typename T, int RT, int MT, bool ALIGNED>
 __global__ __launch_bounds__(64 * kWaves) void adapters_shrink_kernel(const T *__restrict__ X, const T *__restrict__ A,
                                                                       const int *__restrict__ ptr,
                                                                       const int *__restrict__ row_of,
                                                                       float *__restrict__ V, AdaptersShape sh)
 {
     constexpr int C = 16 / sizeof(T), STEP = 4 * C;
-    __shared__ float4v join[kWaves - 1][RT][64];
-    const RowTile t = find_row_tile<kRows>(ptr, sh.E, sh.T, blockIdx.x);
+    __shared__ float4v join[kWaves][RT][64];
+    const RowTile t = find_row_tile<16 * MT>(ptr, sh.E, sh.T, blockIdx.x);
     if (t.rows == 0) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i = lane & 15, g = lane >> 4;
-    int token = i < t.rows ? row_of[t.first + i] : -1;
-    if ((unsigned)token >= (unsigned)sh.T) token = -1;
-    const T *x = X + (size_t)(token < 0 ? 0 : token) * sh.K;
-    const T *a = A + (size_t)t.expert * sh.R * sh.K;
-    const int k0 = blockIdx.y * sh.per_split, k1 = min(k0 + sh.per_split, sh.K);
-    float4v acc[RT] = {};
-    for (int k = k0 + wave * STEP + g * C; k - g * C < k1; k += kWaves * STEP) {
-        const uint4v q = load_chunk<T, ALIGNED>(x + k, token < 0 ? 0 : k1 - k);
+    const T *x[MT];
+    bool live[MT];
 #pragma unroll
-        for (int n = 0; n < RT; ++n) {
-            const int r = n * 16 + i;
-            const uint4v p = load_chunk<T, ALIGNED>(a + (size_t)(r < sh.R ? r : 0) * sh.K + k, r < sh.R ? k1 - k : 0);
-            acc[n] = mma<T>(p, q, acc[n]);
+    for (int m = 0; m < MT; ++m) {
+        const int token = 16 * m + i < t.rows ? row_of[t.first + 16 * m + i] : -1;
+        live[m] = (unsigned)token < (unsigned)sh.T;
+        x[m] = X + (size_t)(live[m] ? token : 0) * sh.K;
+    }
+    const T *a[RT];
+#pragma unroll
+    for (int n = 0; n < RT; ++n) {
+        const int r = n * 16 + i;
+        a[n] = A + ((size_t)t.expert * sh.R + (r < sh.R ? r : 0)) * sh.K;
+    }
+    const int k0 = blockIdx.y * sh.per_split, k1 = min(k0 + sh.per_split, sh.K);
+    float4v acc[MT][RT] = {};
+    for (int base = k0 + wave * 2 * STEP; base < k1; base += kWaves * 2 * STEP) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int k = base + half * STEP + g * C;
+            uint4v q[MT], p[RT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) q[m] = load_chunk<T, ALIGNED>(x[m] + k, live[m] ? k1 - k : 0);
+#pragma unroll
+            for (int n = 0; n < RT; ++n) p[n] = load_chunk<T, ALIGNED>(a[n] + k, n * 16 + i < sh.R ? k1 - k : 0);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < RT; ++n) acc[m][n] = mma<T>(p[n], q[m], acc[m][n]);
         }
     }
-    if (wave > 0) {
+    // The wavefronts' sums meet 16 tokens at a time; each wavefront adds a share of the ranks up.
 #pragma unroll
-        for (int n = 0; n < RT; ++n) join[wave - 1][n][lane] = acc[n];
-    }
-    __syncthreads();
-    if (wave == 0 && i < t.rows) {
-        float *out = V + ((size_t)blockIdx.y * sh.T + t.first + i) * sh.padded + g * 4;
+    for (int m = 0; m < MT; ++m) {
+        if (m > 0) __syncthreads();
 #pragma unroll
-        for (int n = 0; n < RT; ++n) {
-            float4v sum = acc[n];
+        for (int n = 0; n < RT; ++n) join[wave][n][lane] = acc[m][n];
+        __syncthreads();
+        if (16 * m + i < t.rows) {
+            float *out = V + ((size_t)blockIdx.y * sh.T + t.first + 16 * m + i) * sh.padded + g * 4;
+            for (int n = wave; n < RT; n += kWaves) {
+                float4v sum = join[0][n][lane];
 #pragma unroll
-            for (int w = 0; w < kWaves - 1; ++w) sum += join[w][n][lane];
-            *reinterpret_cast<float4v *>(out + n * 16) = sum;
+                for (int w = 1; w < kWaves; ++w) sum += join[w][n][lane];
+                *reinterpret_cast<float4v *>(out + n * 16) = sum;
+            }
         }
     }
 }
 
-// One workgroup per tile of 16 tokens and 256 columns, a wavefront 64 columns.
-// V is made in fp32; for the product with B it is split into its rounding to T
-// and the rounding of what that leaves, two instructions instead of one, so
-// that it is not rounded to 8 or 11 bits on the way.  fp16 has no room for
-// values from 65520 on: where a tile holds one, all of its V are taken down by
-// 2^16 and the sums up again.  RANK: the largest rank, in units of 32.
-template <typename T, int RANK, bool ALIGNED>
+// One workgroup per tile of 16 MT tokens and `columns` columns; a wavefront takes
+// 64 columns at a time, with the tokens' V in its registers throughout.  V is
+// made in fp32; for the product with B it is split into its rounding to T and
+// the rounding of what that leaves, two instructions instead of one, so that
+// it is not rounded to 8 or 11 bits on the way.  fp16 has no room for values
+// from 65520 on: where a tile holds one, all of its V are taken down by 2^16
+// and the sums up again.  RANK: the largest rank, in units of 32.
+// Row g * 4 + d of the b-th matrix instruction is column g * 16 + b * 4 + d, so
+// that a lane ends up with 16 neighbouring columns of a token.
+template <typename T, int RANK, int MT, bool ALIGNED>
 __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const float *__restrict__ V,
                                                                       const T *__restrict__ B,
                                                                       const float *__restrict__ scale, const T *base,
                                                                       T *Y, const int *__restrict__ ptr,
-                                                                      const int *__restrict__ row_of, AdaptersShape sh)
+                                                                      const int *__restrict__ row_of, int columns,
+                                                                      AdaptersShape sh)
 {
-    constexpr int C = 16 / sizeof(T), STEP = 4 * C;
+    constexpr int C = 16 / sizeof(T), STEP = 4 * C, STEPS = RANK * 32 / STEP, ROWS = 16 * MT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i = lane & 15, g = lane >> 4;
     // The tokens without an adapter are one more segment, of which only the base is left.
     const int routed = clamp_place(ptr[sh.E], sh.T);
-    const int tail_tiles = (sh.T - routed + kRows - 1) / kRows;
+    const int tail_tiles = (sh.T - routed + ROWS - 1) / ROWS;
     RowTile t;
     if ((int)blockIdx.y < tail_tiles) {
         t.expert = -1;
-        t.first = routed + blockIdx.y * kRows;
-        t.rows = min(sh.T - t.first, kRows);
+        t.first = routed + blockIdx.y * ROWS;
+        t.rows = min(sh.T - t.first, ROWS);
     } else {
-        t = find_row_tile<kRows>(ptr, sh.E, sh.T, blockIdx.y - tail_tiles);
+        t = find_row_tile<ROWS>(ptr, sh.E, sh.T, blockIdx.y - tail_tiles);
         if (t.rows == 0) return;
     }
-    const int token = i < t.rows ? row_of[t.first + i] : -1;
-    const bool live = (unsigned)token < (unsigned)sh.T;
-    const int n0 = (blockIdx.x * kWaves + wave) * 64;
-    if (n0 >= sh.N) return;
-    float4v acc[4] = {};
+    int token[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        token[m] = 16 * m + i < t.rows ? row_of[t.first + 16 * m + i] : -1;
+        if ((unsigned)token[m] >= (unsigned)sh.T) token[m] = -1;
+    }
+    uint4v high[MT][STEPS], low[MT][STEPS];
+    bool taken[MT] = {};  // down by 2^16
     if (t.expert >= 0) {
         const float s = scale ? scale[t.expert] : 1.0f;
-        const T *b = B + (size_t)t.expert * sh.N * sh.R;
-        constexpr int STEPS = RANK * 32 / STEP;
-        float v[STEPS][C];
-        bool far = false;
 #pragma unroll
-        for (int m = 0; m < STEPS; ++m) {
-            const int r = m * STEP + g * C;
+        for (int m = 0; m < MT; ++m) {
+            float v[STEPS][C];
+            bool far = false;
 #pragma unroll
-            for (int c = 0; c < C; ++c) v[m][c] = 0.0f;
-            if (live && r < sh.padded) {
-                for (int part = 0; part < sh.splits; ++part) {
-                    const float *from = V + ((size_t)part * sh.T + t.first + i) * sh.padded + r;
+            for (int step = 0; step < STEPS; ++step) {
+                const int r = step * STEP + g * C;
 #pragma unroll
-                    for (int c = 0; c < C; c += 4) {
-                        const float4v f = *reinterpret_cast<const float4v *>(from + c);
+                for (int c = 0; c < C; ++c) v[step][c] = 0.0f;
+                if (token[m] >= 0 && r < sh.padded) {
+                    for (int part = 0; part < sh.splits; ++part) {
+                        const float *from = V + ((size_t)part * sh.T + t.first + 16 * m + i) * sh.padded + r;
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) v[m][c + d] += f[d];
+                        for (int c = 0; c < C; c += 4) {
+                            const float4v f = *reinterpret_cast<const float4v *>(from + c);
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) v[step][c + d] += f[d];
+                        }
                     }
                 }
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    v[step][c] = r + c < sh.R ? v[step][c] * s : 0.0f;  // infinite rows have NaN behind the rank
+                    far |= __builtin_fabsf(v[step][c]) > 65000.0f;
+                }
             }
+            // 16 tokens share a scale; the other 16s of a tile have their own
+            const bool take = __is_same(T, half_t) && __any(far);
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                v[m][c] = r + c < sh.R ? v[m][c] * s : 0.0f;  // infinite rows have NaN behind the rank
-                far |= __builtin_fabsf(v[m][c]) > 65000.0f;
+            for (int step = 0; step < STEPS; ++step) {
+                T high_of[C], low_of[C];
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const float x = take ? v[step][c] * 0x1p-16f : v[step][c];
+                    high_of[c] = (T)x;
+                    const float rest = x - (float)high_of[c];
+                    low_of[c] = (T)(__builtin_fabsf(rest) < __builtin_inff() ? rest : 0.0f);  // infinities stand in `high`
+                }
+                __builtin_memcpy(&high[m][step], high_of, 16);
+                __builtin_memcpy(&low[m][step], low_of, 16);
             }
-        }
-        const bool down = __is_same(T, half_t) && __any(far);
-#pragma unroll
-        for (int m = 0; m < STEPS; ++m) {
-            const int r = m * STEP + g * C;
-            if (m * STEP >= sh.R) break;
-            uint4v high, low;
-            T high_of[C], low_of[C];
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const float x = down ? v[m][c] * 0x1p-16f : v[m][c];
-                high_of[c] = (T)x;
-                const float rest = x - (float)high_of[c];
-                low_of[c] = (T)(__builtin_fabsf(rest) < __builtin_inff() ? rest : 0.0f);  // infinities stand in `high`
-            }
-            __builtin_memcpy(&high, high_of, 16);
-            __builtin_memcpy(&low, low_of, 16);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const int col = n0 + n * 16 + i;
-                const uint4v p = load_chunk<T, ALIGNED>(b + (size_t)(col < sh.N ? col : 0) * sh.R + r,
-                                                        col < sh.N ? sh.R - r : 0);
-                acc[n] = mma<T>(p, high, acc[n]);
-                if constexpr (sizeof(T) == 2) acc[n] = mma<T>(p, low, acc[n]);
-            }
-        }
-        if (down) {
-#pragma unroll
-            for (int n = 0; n < 4; ++n) acc[n] *= 65536.0f;
+            taken[m] = take;
         }
     }
-    if (!live) return;
+    const T *b_of = B + (size_t)max(t.expert, 0) * sh.N * sh.R;
+    for (int n0 = blockIdx.x * columns + wave * 64; n0 < min((int)(blockIdx.x + 1) * columns, sh.N); n0 += kWaves * 64) {
+        float4v acc[MT][4] = {};
+        if (t.expert >= 0) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-        const int col = n0 + n * 16 + g * 4;
-        if (col >= sh.N) continue;
-        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (base) load_vec<T, 4, ALIGNED>(y, base + (size_t)token * sh.N + col, sh.N - col);
+            for (int step = 0; step < STEPS; ++step) {
+                if (step * STEP >= sh.R) break;
+                const int r = step * STEP + g * C;
+                uint4v p[4];
 #pragma unroll
-        for (int d = 0; d < 4; ++d) y[d] += acc[n][d];
-        store_vec<T, 4, ALIGNED>(Y + (size_t)token * sh.N + col, y, sh.N - col);
+                for (int b = 0; b < 4; ++b) {
+                    const int col = n0 + (i >> 2) * 16 + b * 4 + (i & 3);
+                    p[b] = load_chunk<T, ALIGNED>(b_of + (size_t)(col < sh.N ? col : 0) * sh.R + r, col < sh.N ? sh.R - r : 0);
+                }
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        acc[m][b] = mma<T>(p[b], high[m][step], acc[m][b]);
+                        if constexpr (sizeof(T) == 2) acc[m][b] = mma<T>(p[b], low[m][step], acc[m][b]);
+                    }
+            }
+        }
+        const int col = n0 + g * 16;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (token[m] < 0 || col >= sh.N) continue;
+            const size_t at = (size_t)token[m] * sh.N + col;
+            const float up = __is_same(T, half_t) && taken[m] ? 65536.0f : 1.0f;
+#pragma unroll
+            for (int b = 0; b < 16; b += C) {
+                if (col + b >= sh.N) break;
+                float y[C];
+#pragma unroll
+                for (int c = 0; c < C; ++c) y[c] = 0.0f;
+                if (base) load_vec<T, C, ALIGNED>(y, base + at + b, sh.N - col - b);
+#pragma unroll
+                for (int c = 0; c < C; ++c) y[c] += acc[m][(b + c) / 4][(b + c) % 4] * up;
+                store_vec<T, C, ALIGNED>(Y + at + b, y, sh.N - col - b);
+            }
+        }
     }
 }
 
@@ -214,10 +259,10 @@ AdaptersShape make_shape(int T, int E, int R, int K, int N)
 {
     int padded = 16;
     while (padded < R) padded *= 2;
-    AdaptersShape sh{T, E, R, K, N, padded, 1, K};
-    // Parts of the sum over K: about 1024 workgroups, each with at least 256 of K.
-    const long long tiles = num_row_tiles(T, E < T ? E : T, kRows);
-    long long splits = 1024 / (tiles > 0 ? tiles : 1);
+    AdaptersShape sh{T, E, R, K, N, padded, 1, K, T >= 128LL * E};
+    // Parts of the sum over K: about 512 workgroups, each with at least 256 of K.
+    const long long tiles = num_row_tiles(T, E < T ? E : T, sh.tall ? 64 : 16);
+    long long splits = (512 + tiles - 1) / (tiles > 0 ? tiles : 1);
     if (splits > K / 256) splits = K / 256;
     if (splits > 16) splits = 16;
     if (splits < 1) splits = 1;
@@ -226,38 +271,68 @@ AdaptersShape make_shape(int T, int E, int R, int K, int N)
     return sh;
 }
 
-template <typename T>
-int launch_adapters(const void *X, const void *A, const void *B, const float *scale, const void *base, void *Y,
-                    const int *ptr, const int *row_of, const AdaptersShape &sh, float *V, hipStream_t st)
+// MT of the two kernels: what fits the registers beside the rank.
+constexpr int shrink_tiles(int RT) { return RT <= 4 ? 4 : RT == 8 ? 2 : 1; }
+constexpr int expand_tiles(int RANK) { return RANK <= 2 ? 4 : 1; }
+
+template <typename T, int RT, int MT>
+int launch_shrink(const T *X, const T *A, const int *ptr, const int *row_of, float *V, const AdaptersShape &sh,
+                  hipStream_t st)
 {
-    const long long tiles = num_row_tiles(sh.T, sh.E, kRows);
-    const dim3 shrink((unsigned)tiles, sh.splits);
-    const bool fast = rows_of_16(X, sh.K, sizeof(T)) && rows_of_16(A, sh.K, sizeof(T));
-#define MPS_LAUNCH_SHRINK(RT)                                                                                       \
-    if (fast)                                                                                                       \
-        hipLaunchKernelGGL((adapters_shrink_kernel<T, RT, true>), shrink, dim3(64 * kWaves), 0, st,                 \
-                           static_cast<const T *>(X), static_cast<const T *>(A), ptr, row_of, V, sh);               \
-    else                                                                                                            \
-        hipLaunchKernelGGL((adapters_shrink_kernel<T, RT, false>), shrink, dim3(64 * kWaves), 0, st,                \
-                           static_cast<const T *>(X), static_cast<const T *>(A), ptr, row_of, V, sh)
-    if (sh.padded <= 16) { MPS_LAUNCH_SHRINK(1); }
-    else if (sh.padded <= 32) { MPS_LAUNCH_SHRINK(2); }
-    else if (sh.padded <= 64) { MPS_LAUNCH_SHRINK(4); }
-    else if (sh.padded <= 128) { MPS_LAUNCH_SHRINK(8); }
-    else { MPS_LAUNCH_SHRINK(16); }
-#undef MPS_LAUNCH_SHRINK
-    MPS_HIP_TRY(hipGetLastError());
-    const dim3 expand(ceil_div(sh.N, 64 * kWaves), (unsigned)tiles + 1);
-    const bool fast2 = rows_of_16(B, sh.R, sizeof(T)) && rows_of_16(base, sh.N, sizeof(T)) && rows_of_16(Y, sh.N, sizeof(T));
-#define MPS_LAUNCH_EXPAND(RANK, ALIGNED)                                                                             \
-    hipLaunchKernelGGL((adapters_expand_kernel<T, RANK, ALIGNED>), expand, dim3(64 * kWaves), 0, st, V,                    \
-                       static_cast<const T *>(B), scale, static_cast<const T *>(base), static_cast<T *>(Y), ptr, row_of, sh)
-    if (sh.R <= 32) { if (fast2) MPS_LAUNCH_EXPAND(1, true); else MPS_LAUNCH_EXPAND(1, false); }
-    else if (sh.R <= 64) { if (fast2) MPS_LAUNCH_EXPAND(2, true); else MPS_LAUNCH_EXPAND(2, false); }
-    else { if (fast2) MPS_LAUNCH_EXPAND(8, true); else MPS_LAUNCH_EXPAND(8, false); }
-#undef MPS_LAUNCH_EXPAND
+    const dim3 grid((unsigned)num_row_tiles(sh.T, sh.E, 16 * MT), sh.splits);
+    if (rows_of_16(X, sh.K, sizeof(T)) && rows_of_16(A, sh.K, sizeof(T)))
+        hipLaunchKernelGGL((adapters_shrink_kernel<T, RT, MT, true>), grid, dim3(64 * kWaves), 0, st, X, A, ptr, row_of, V, sh);
+    else
+        hipLaunchKernelGGL((adapters_shrink_kernel<T, RT, MT, false>), grid, dim3(64 * kWaves), 0, st, X, A, ptr, row_of, V, sh);
     MPS_HIP_TRY(hipGetLastError());
     return MPS_OK;
+}
+
+template <typename T, int RANK, int MT>
+int launch_expand(const float *V, const T *B, const float *scale, const T *base, T *Y, const int *ptr, const int *row_of,
+                  const AdaptersShape &sh, hipStream_t st)
+{
+    const long long tiles = num_row_tiles(sh.T, sh.E, 16 * MT) + 1;
+    // Columns of a workgroup: as many as leave about 1024 of them, at most 1024, so that V is not read too often.
+    long long columns = (long long)sh.N * tiles / 1024 / 256 * 256;
+    columns = columns < 256 ? 256 : columns > 1024 ? 1024 : columns;
+    const dim3 grid(ceil_div(sh.N, columns), (unsigned)tiles);
+    const bool fast = rows_of_16(B, sh.R, sizeof(T)) && rows_of_16(base, sh.N, sizeof(T)) && rows_of_16(Y, sh.N, sizeof(T));
+    if (fast)
+        hipLaunchKernelGGL((adapters_expand_kernel<T, RANK, MT, true>), grid, dim3(64 * kWaves), 0, st, V, B, scale, base,
+                           Y, ptr, row_of, (int)columns, sh);
+    else
+        hipLaunchKernelGGL((adapters_expand_kernel<T, RANK, MT, false>), grid, dim3(64 * kWaves), 0, st, V, B, scale, base,
+                           Y, ptr, row_of, (int)columns, sh);
+    MPS_HIP_TRY(hipGetLastError());
+    return MPS_OK;
+}
+
+template <typename T>
+int launch_adapters(const void *X_, const void *A_, const void *B_, const float *scale, const void *base_, void *Y_,
+                    const int *ptr, const int *row_of, const AdaptersShape &sh, float *V, hipStream_t st)
+{
+    const T *X = static_cast<const T *>(X_), *A = static_cast<const T *>(A_), *B = static_cast<const T *>(B_);
+    const T *base = static_cast<const T *>(base_);
+    T *Y = static_cast<T *>(Y_);
+    int rc;
+#define MPS_SHRINK(RT)                                                                                 \
+    rc = sh.tall ? launch_shrink<T, RT, shrink_tiles(RT)>(X, A, ptr, row_of, V, sh, st)                \
+                 : launch_shrink<T, RT, 1>(X, A, ptr, row_of, V, sh, st)
+    if (sh.padded <= 16) MPS_SHRINK(1);
+    else if (sh.padded <= 32) MPS_SHRINK(2);
+    else if (sh.padded <= 64) MPS_SHRINK(4);
+    else if (sh.padded <= 128) MPS_SHRINK(8);
+    else MPS_SHRINK(16);
+#undef MPS_SHRINK
+    if (rc != MPS_OK) return rc;
+#define MPS_EXPAND(RANK)                                                                                         \
+    return sh.tall ? launch_expand<T, RANK, expand_tiles(RANK)>(V, B, scale, base, Y, ptr, row_of, sh, st)       \
+                   : launch_expand<T, RANK, 1>(V, B, scale, base, Y, ptr, row_of, sh, st)
+    if (sh.R <= 32) MPS_EXPAND(1);
+    if (sh.R <= 64) MPS_EXPAND(2);
+    MPS_EXPAND(8);
+#undef MPS_EXPAND
 }
 
 int check_adapters(int T, int E, int R, int K)

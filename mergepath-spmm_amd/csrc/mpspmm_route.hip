@@ -4,6 +4,9 @@
 // gradients.
 #include "mpspmm_routing.hpp"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace {
 
 constexpr int kRouteBlock = 256;
@@ -40,20 +43,10 @@ __device__ __forceinline__ double of_key(unsigned long long k)
     if (k == 0) return -__builtin_inf();
     return __builtin_bit_cast(double, k >> 63 ? k & 0x7FFFFFFFFFFFFFFFull : ~k);
 }
-template <typename S>
-struct KeyOf;
-template <>
-struct KeyOf<float> {
-    using type = unsigned;
-};
-template <>
-struct KeyOf<double> {
-    using type = unsigned long long;
-};
-
 struct RouteShape {
     int T, E, k, score, groups, group_size, top_groups, group_score, renormalise;
     float scale;
+    int group_lanes;  // lanes that hold a group's experts, a power of two; 0: groups and lanes do not fit each other
 };
 
 // exp(x), x <= 0 in the softmax: the rounding of x * log2(e) is made good by
@@ -73,42 +66,256 @@ __device__ __forceinline__ float sigmoid_near(float l)
     const float r = 1.0f / (1.0f + e);
     return l != l ? l : (l >= 0.0f ? r : e * r);
 }
-__device__ __forceinline__ double sigmoid_f64(double l) { return 1.0 / (1.0 + exp(-l)); }
 
-// How far two choice scores formed in 32 bits may be off together: the score
-// itself by less than 2^-22 (see exp_near; sigmoid and softmax are at most
-// 1), the sum with the bias by half a step.  Twice that, for both sides, and
-// some room.
-__device__ __forceinline__ float doubt(float a, float b)
+// What a chosen score l counts beside the others, up to a factor that is the
+// same for all of a token; top = the largest of them.  0 for a slot without one.
+__device__ __forceinline__ float chosen_share(float l, float top, bool soft)
 {
-    return 0x1p-20f * fmaxf(1.0f, fmaxf(__builtin_fabsf(a), __builtin_fabsf(b)));
+    if (l == -__builtin_inff()) return 0.0f;
+    if (l != l) return l;
+    float p = l == top ? 1.0f : exp_near(l - top);  // infinite ones too
+    // sigmoid(l), or where all are small sigmoid(l) * exp(-top): neither overflows, nor vanishes at the top
+    if (!soft) p = top > 0.0f ? sigmoid_near(l) : p / (1.0f + exp_near(l));
+    return p;
 }
 
-// The k best of a token's keys, held by L lanes with IPL experts each (expert
-// lane * IPL + i).  The j-th choice ends up in lane j.  With WATCH, returns
-// true where a decision was closer than 32 bits can tell.
-template <typename S, int IPL, int L, bool WATCH>
-__device__ __forceinline__ bool choose(typename KeyOf<S>::type (&key)[IPL], const RouteShape &sh, int lane,
-                                       int &chosen_expert)
+// LDS that only one wavefront uses: its operations happen in order.
+__device__ __forceinline__ void wave_sync()
 {
-    using Key = typename KeyOf<S>::type;
-    const int group_base = (threadIdx.x & 63) & ~(L - 1);
-    bool close = false;
-    Key last = 0;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// exp(x) for x <= 0 to about 2^-46 of itself: 2^n times the first twelve terms of
+// the series at |r| <= log(2) / 2, whose remainder is r^12 / 12! < 7e-15.
+__device__ __forceinline__ double exp_wide(double x)
+{
+    const double n = __builtin_rint(x * 1.4426950408889634074);
+    double r = __builtin_fma(n, -6.93147180369123816490e-01, x);  // the first 32 bits of log(2), and the rest
+    r = __builtin_fma(n, -1.90821492927058770002e-10, r);
+    double p = 1.0 / 39916800.0;
+    p = __builtin_fma(p, r, 1.0 / 3628800.0);
+    p = __builtin_fma(p, r, 1.0 / 362880.0);
+    p = __builtin_fma(p, r, 1.0 / 40320.0);
+    p = __builtin_fma(p, r, 1.0 / 5040.0);
+    p = __builtin_fma(p, r, 1.0 / 720.0);
+    p = __builtin_fma(p, r, 1.0 / 120.0);
+    p = __builtin_fma(p, r, 1.0 / 24.0);
+    p = __builtin_fma(p, r, 1.0 / 6.0);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    return x > -700.0 ? __builtin_ldexp(p, (int)n) : x != x ? x : 0.0;
+}
+// 1 / x, 1 <= x <= 2^11: the instruction's estimate, and two of Newton's steps.
+__device__ __forceinline__ double reciprocal_wide(double x)
+{
+    double y = __builtin_amdgcn_rcp(x);
+    y = __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+    return __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+}
+
+// A choice score and its expert in one double, so that one maximum finds the
+// larger score and, of equal ones, the lower expert.  The last 10 bits hold the
+// expert or its complement, whichever counts the right way round for the sign;
+// a score made from one float has zeros there.  NaN and the infinities, which a
+// maximum of doubles would not order, become the largest numbers there are.
+constexpr unsigned kNeverChosen = 0xFFEFFFFFu;  // high word of -inf's stand-in
+constexpr unsigned kInfinite = 0x7FEFFFFEu, kNotANumber = 0x7FEFFFFFu;
+__device__ __forceinline__ double from_words(unsigned hi, unsigned lo)
+{
+    return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ unsigned high_word(double v) { return (unsigned)(__builtin_bit_cast(unsigned long long, v) >> 32); }
+__device__ __forceinline__ unsigned low_word(double v) { return (unsigned)__builtin_bit_cast(unsigned long long, v); }
+__device__ __forceinline__ double pack_choice(double c, int expert)
+{
+    c += 0.0;  // -0 ranks as +0
+    unsigned hi = high_word(c), lo = low_word(c);
+    if (!(__builtin_fabs(c) < __builtin_inf())) {
+        hi = c != c ? kNotANumber : c > 0.0 ? kInfinite : kNeverChosen;
+        lo = 0;
+    }
+    const unsigned tag = (unsigned)(hi >> 31 ? expert : ~expert) & 1023u;
+    return from_words(hi, (lo & ~1023u) | tag);
+}
+__device__ __forceinline__ int expert_of(double v)
+{
+    return (int)((high_word(v) >> 31 ? low_word(v) : ~low_word(v)) & 1023u);
+}
+// As written, without the steps that the compiler adds for NaN: there are none.
+__device__ __forceinline__ double max_f64(double a, double b)
+{
+    double r;
+    asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ double min_f64(double a, double b)
+{
+    double r;
+    asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+template <int L>
+__device__ __forceinline__ double group_max_f64(double v)
+{
+    if constexpr (L > 1) v = max_f64(v, lane_partner_f64<1>(v));
+    if constexpr (L > 2) v = max_f64(v, lane_partner_f64<2>(v));
+    if constexpr (L > 4) v = max_f64(v, lane_partner_f64<4>(v));
+    if constexpr (L > 8) v = max_f64(v, lane_partner_f64<8>(v));
+    if constexpr (L > 16) v = max_f64(v, lane_partner_f64<16>(v));
+    if constexpr (L > 32) v = max_f64(v, lane_partner_f64<32>(v));
+    return v;
+}
+
+// How near two packed choice scores may be and still not be told apart: a score
+// is off by 2^-44 of one at most, the tag by 2^-42 of the whole.
+__device__ __forceinline__ double doubt(double a, double b)
+{
+    return 0x1p-38 * __builtin_fmax(1.0, __builtin_fmax(__builtin_fabs(a), __builtin_fabs(b)));
+}
+
+// The k best of a token's packed choice scores, held by L lanes with IPL experts
+// each (expert lane * IPL + i).  The j-th choice ends up in lane j.  With
+// WATCH the (k + 1)-th too; returned are the places j whose choice is too near
+// the one before it.
+template <int IPL, int L, bool WATCH>
+__device__ __forceinline__ unsigned long long choose(double (&v)[IPL], int k, int lane, int &chosen_expert)
+{
+    unsigned long long close = 0;
+    double last = 0.0;
     chosen_expert = -1;
-    for (int j = 0; j < sh.k + (WATCH ? 1 : 0); ++j) {
-        Key m = key[0];
+    for (int j = 0; j < k + (WATCH ? 1 : 0); ++j) {
+        double m[IPL];
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) m[i] = v[i];
+#pragma unroll
+        for (int step = 1; step < IPL; step *= 2)
+#pragma unroll
+            for (int i = 0; i + step < IPL; i += 2 * step) m[i] = max_f64(m[i], m[i + step]);
+        const double best = group_max_f64<L>(m[0]);
+        const bool is = high_word(best) != kNeverChosen;
+        if constexpr (WATCH) {
+            if (j > 0 && is && last - best <= doubt(last, best)) close |= 1ull << j;
+            last = best;
+        }
+        const int e = expert_of(best);
+        if (lane == j) chosen_expert = is ? e : -1;
+        const int mine = e - lane * IPL;
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) v[i] = from_words(i == mine ? kNeverChosen : high_word(v[i]), low_word(v[i]));
+    }
+    return close;
+}
+
+// Drops the experts outside the top_groups best groups where a group's experts
+// lie in group_lanes whole lanes.  Returns whether that was too near to tell.
+template <int IPL, int L, bool WATCH>
+__device__ __forceinline__ bool keep_group_lanes(double (&v)[IPL], const RouteShape &sh, int lane,
+                                                 double *__restrict__ of_group)
+{
+    double first = v[0], second = from_words(kNeverChosen, 0);
+#pragma unroll
+    for (int i = 1; i < IPL; ++i) {
+        second = max_f64(second, min_f64(first, v[i]));
+        first = max_f64(first, v[i]);
+    }
+#define MPS_MERGE_STEP(STEP)                                                                        \
+    if constexpr (L > STEP) {                                                                       \
+        if (sh.group_lanes > STEP) {                                                                \
+            const double f = lane_partner_f64<STEP>(first), g = lane_partner_f64<STEP>(second);     \
+            second = max_f64(min_f64(first, f), max_f64(second, g));                                \
+            first = max_f64(first, f);                                                              \
+        }                                                                                           \
+    }
+    MPS_MERGE_STEP(1) MPS_MERGE_STEP(2) MPS_MERGE_STEP(4) MPS_MERGE_STEP(8) MPS_MERGE_STEP(16) MPS_MERGE_STEP(32)
+#undef MPS_MERGE_STEP
+    // the largest members carry their experts' numbers, so that of equal groups the lower is larger
+    const double own = sh.group_score == MPS_GROUP_TOP2 ? first + second : first;
+    const int group = lane / sh.group_lanes;
+    if (group < sh.groups && lane % sh.group_lanes == 0) of_group[group] = own;
+    wave_sync();
+    int better = 0, near = 0;
+    for (int h = 0; h < sh.groups; ++h) {
+        const double x = of_group[h];
+        better += x > own || (x == own && h < group);
+        // two groups without experts are equally bad (their difference is NaN)
+        if constexpr (WATCH) near += h != group && __builtin_fabs(x - own) <= 2.0 * doubt(x, own);
+    }
+    wave_sync();
+    if (better >= sh.top_groups || group >= sh.groups) {
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) v[i] = from_words(kNeverChosen, low_word(v[i]));
+    }
+    // a kept group that might be behind the border; a group behind it that might be kept is near one
+    return WATCH && group < sh.groups && better < sh.top_groups && better + near >= sh.top_groups;
+}
+
+// The same choice without shortcuts, with scores in 64 bits and ties by index:
+// for tokens that the above leaves in doubt, and for groups that do not fit the
+// lanes.  `all`: sh.E scores of LDS, `of_group`: sh.groups.
+template <typename T, int IPL, int L>
+__device__ __forceinline__ int choose_again(const T *__restrict__ row, bool live, const float *__restrict__ bias,
+                                            const RouteShape &sh, int lane, bool plain, float largest,
+                                            unsigned long long *__restrict__ all, unsigned long long *__restrict__ of_group)
+{
+    const bool soft = sh.score == MPS_SCORE_SOFTMAX;
+    const float minus_inf = -__builtin_inff();
+    double sum = 0.0;
+    if (soft && !plain) {
+#pragma unroll 1
+        for (int i = 0; i < IPL; ++i) {
+            const int x = lane * IPL + i;
+            const float l = live && x < sh.E ? (float)row[x] : minus_inf;
+            if (l != minus_inf) sum += exp((double)l - (double)largest);
+        }
+        sum = group_sum<L>(sum);
+    }
+    unsigned long long key[IPL];
+#pragma unroll
+    for (int i = 0; i < IPL; ++i) {
+        const int x = lane * IPL + i;
+        const float l = live && x < sh.E ? (float)row[x] : minus_inf;
+        double c = (double)l;
+        if (!plain && l != minus_inf) {
+            c = soft ? exp(c - (double)largest) / sum : 1.0 / (1.0 + exp(-c));
+            if (bias) c += (double)bias[x];
+        }
+        key[i] = key_of(c);
+    }
+    if (sh.groups > 1) {
+#pragma unroll
+        for (int i = 0; i < IPL; ++i)
+            if (lane * IPL + i < sh.E) all[lane * IPL + i] = key[i];
+        wave_sync();
+        for (int g = lane; g < sh.groups; g += L) {
+            unsigned long long first = 0, second = 0;
+            for (int i = 0; i < sh.group_size; ++i) {
+                const unsigned long long v = all[g * sh.group_size + i];
+                second = max(second, min(first, v));
+                first = max(first, v);
+            }
+            of_group[g] = sh.group_score == MPS_GROUP_TOP2 ? key_of(of_key(first) + of_key(second)) : first;
+        }
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) {
+            const int g = min((lane * IPL + i) / sh.group_size, sh.groups - 1);
+            const unsigned long long own = of_group[g];
+            int better = 0;
+            for (int h = 0; h < sh.groups; ++h) better += of_group[h] > own || (of_group[h] == own && h < g);
+            if (better >= sh.top_groups) key[i] = 0;
+        }
+        wave_sync();
+    }
+    const int group_base = (threadIdx.x & 63) & ~(L - 1);
+    int chosen_expert = -1;
+    for (int j = 0; j < sh.k; ++j) {
+        unsigned long long m = key[0];
 #pragma unroll
         for (int i = 1; i < IPL; ++i) m = max(m, key[i]);
-        const Key best = group_max<L>(m);
-        if constexpr (WATCH) {
-            if (j > 0 && best != 0) {
-                const float a = (float)of_key(last), b = (float)of_key(best);
-                close |= a - b <= doubt(a, b);
-            }
-            last = best;
-            if (j == sh.k) break;
-        }
+        const unsigned long long best = group_max<L>(m);
         const unsigned long long has = __ballot(m == best) >> group_base;
         const int owner = __ffsll(L == 64 ? has : has & ((1ull << L) - 1)) - 1;
         int at = -1;
@@ -123,93 +330,29 @@ __device__ __forceinline__ bool choose(typename KeyOf<S>::type (&key)[IPL], cons
         const int e = __shfl(lane * IPL + at, group_base + owner, 64);
         if (lane == j) chosen_expert = best != 0 ? e : -1;
     }
-    return close;
+    return chosen_expert;
 }
 
-// Zeroes the keys of the experts outside the top_groups best groups.  `mine`:
-// this token's part of LDS, 2 * groups values of S.
-template <typename S, int IPL, int L, bool WATCH>
-__device__ __forceinline__ bool keep_groups(typename KeyOf<S>::type (&key)[IPL], const RouteShape &sh, int lane,
-                                            typename KeyOf<S>::type *__restrict__ all,
-                                            typename KeyOf<S>::type *__restrict__ of_group)
-{
-    using Key = typename KeyOf<S>::type;
-#pragma unroll
-    for (int i = 0; i < IPL; ++i)
-        if (lane * IPL + i < sh.E) all[lane * IPL + i] = key[i];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    for (int g = lane; g < sh.groups; g += L) {
-        Key first = 0, second = 0;
-        for (int i = 0; i < sh.group_size; ++i) {
-            const Key v = all[g * sh.group_size + i];
-            second = max(second, min(first, v));
-            first = max(first, v);
-        }
-        of_group[g] = sh.group_score == MPS_GROUP_TOP2 ? key_of((S)(of_key(first) + of_key(second))) : first;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    bool close = false;
-    unsigned long long kept = 0;
-    for (int g = lane; g < sh.groups; g += L) {
-        const Key own = of_group[g];
-        int better = 0, surely = 0;
-        for (int h = 0; h < sh.groups; ++h) {
-            const Key v = of_group[h];
-            better += v > own || (v == own && h < g);
-            if constexpr (WATCH) {
-                // groups that are better by more than the doubt; the others might be worse
-                const float a = (float)of_key(v), b = (float)of_key(own);
-                surely += h != g && v != 0 && own != 0 && __builtin_fabsf(a - b) <= 2.0f * doubt(a, b);
-            }
-        }
-        // in doubt where a group near this one might change its side of the border
-        if (WATCH && surely != 0 && better <= sh.top_groups && better + surely >= sh.top_groups - 1) close = true;
-        if (better < sh.top_groups) kept |= 1ull << g;
-    }
-    unsigned lo = (unsigned)kept, hi = (unsigned)(kept >> 32);
-#define MPS_OR_STEP(STEP)                                  \
-    if constexpr (L > STEP) {                              \
-        lo |= lane_partner<STEP>(lo);                      \
-        hi |= lane_partner<STEP>(hi);                      \
-    }
-    MPS_OR_STEP(1) MPS_OR_STEP(2) MPS_OR_STEP(4) MPS_OR_STEP(8) MPS_OR_STEP(16) MPS_OR_STEP(32)
-#undef MPS_OR_STEP
-    kept = ((unsigned long long)hi << 32) | lo;
-#pragma unroll
-    for (int i = 0; i < IPL; ++i) {
-        const int g = min((lane * IPL + i) / sh.group_size, sh.groups - 1);
-        if (!((kept >> g) & 1)) key[i] = 0;
-    }
-    return close;
-}
-
-// One token by L lanes.  The scores are read once.  Without a bias and without
-// sums over a group c orders as l does, which is exact; else c is formed in 32
-// bits, and a token in which a decision falls by less than their error is done
-// again in 64 bits: the choice is that of 64 bits, at the cost of 32.
+// One token by L > k lanes; lane j gets the j-th choice and its weight.  The
+// scores are read once.  Without a bias and without sums over a group c orders
+// as l does, which is exact; else c is formed to 2^-44, and a token where two
+// choices are nearer than that and have not the same l and bias, which makes
+// them equal, is done again with every bit of a double.
 template <typename T, int IPL, int L>
-__global__ __launch_bounds__(kRouteBlock) void route_kernel(const T *__restrict__ scores, const float *__restrict__ bias,
-                                                            RouteShape sh, int *__restrict__ expert,
-                                                            float *__restrict__ weight)
+__device__ __forceinline__ void route_token(const T *__restrict__ row, bool live, const float *__restrict__ bias,
+                                            const RouteShape &sh, int lane, unsigned long long *__restrict__ mine, int &e,
+                                            float &w)
 {
-    extern __shared__ unsigned long long route_lds[];
-    constexpr int kTokens = kRouteBlock / L;
-    const int lane = threadIdx.x & (L - 1);
-    const int in_block = threadIdx.x / L;
-    const long long t = (long long)blockIdx.x * kTokens + in_block;
-    const bool live = t < sh.T;
-    const T *row = scores + (live ? t : 0) * sh.E;
-    unsigned long long *mine = route_lds + in_block * (sh.E + sh.groups);
-
+    const float minus_inf = -__builtin_inff();
     float l[IPL];
+    {
+        const int valid = live ? sh.E - lane * IPL : 0;
+        if (valid >= IPL) {
+            load_vec<T, IPL, false>(l, row + lane * IPL, valid);
+        } else {
 #pragma unroll
-    for (int i = 0; i < IPL; ++i) {
-        const int e = lane * IPL + i;
-        l[i] = live && e < sh.E ? (float)row[e] : -__builtin_inff();
+            for (int i = 0; i < IPL; ++i) l[i] = i < valid ? (float)row[lane * IPL + i] : minus_inf;
+        }
     }
     const bool plain = bias == nullptr && (sh.groups <= 1 || sh.group_score == MPS_GROUP_MAX);
     const bool soft = sh.score == MPS_SCORE_SOFTMAX;
@@ -219,87 +362,91 @@ __global__ __launch_bounds__(kRouteBlock) void route_kernel(const T *__restrict_
 #pragma unroll
         for (int i = 0; i < IPL; ++i) m = max(m, key_of(l[i]));
         largest = of_key(group_max<L>(m));
-        if (!plain || !sh.renormalise) {
+    }
+    double v[IPL];
+    if (plain) {
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) v[i] = (double)l[i];
+        if (soft && !sh.renormalise) {
             float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < IPL; ++i) sum += l[i] == -__builtin_inff() ? 0.0f : exp_near(l[i] - largest);
+            for (int i = 0; i < IPL; ++i) sum += l[i] == minus_inf ? 0.0f : exp_near(l[i] - largest);
             total = group_sum<L>(sum);
         }
-    }
-    unsigned key[IPL];
-#pragma unroll
-    for (int i = 0; i < IPL; ++i) {
-        float c = l[i];
-        if (!plain && c != -__builtin_inff()) {
-            c = soft ? exp_near(c - largest) / total : sigmoid_near(c);
-            if (bias) c += bias[lane * IPL + i];
-        }
-        key[i] = key_of(c);
-    }
-    int e;
-    bool close = false;
-    if (plain) {
-        if (sh.groups > 1)
-            keep_groups<float, IPL, L, false>(key, sh, lane, reinterpret_cast<unsigned *>(mine),
-                                              reinterpret_cast<unsigned *>(mine) + sh.E);
-        choose<float, IPL, L, false>(key, sh, lane, e);
     } else {
-        if (sh.groups > 1)
-            close = keep_groups<float, IPL, L, true>(key, sh, lane, reinterpret_cast<unsigned *>(mine),
-                                                     reinterpret_cast<unsigned *>(mine) + sh.E);
-        close |= choose<float, IPL, L, true>(key, sh, lane, e);
-        if (__any(close && live)) {
-            double sum = 1.0;
-            if (soft) {
-                sum = 0.0;
+        double sum = 0.0;
 #pragma unroll
-                for (int i = 0; i < IPL; ++i)
-                    if (l[i] != -__builtin_inff()) sum += exp((double)l[i] - (double)largest);
-                sum = group_sum<L>(sum);
-            }
-            unsigned long long key2[IPL];
+        for (int i = 0; i < IPL; ++i) {
+            const double x = soft ? (double)l[i] - (double)largest : -__builtin_fabs((double)l[i]);
+            v[i] = l[i] == minus_inf ? 0.0 : exp_wide(x);
+            if (soft) sum += v[i];
+        }
+        double scale = 1.0;
+        if (soft) {
+            sum = group_sum<L>(sum);
+            scale = 1.0 / sum;
+            total = (float)sum;
+        }
 #pragma unroll
-            for (int i = 0; i < IPL; ++i) {
-                double c = -__builtin_inf();
-                if (l[i] != -__builtin_inff()) {
-                    c = soft ? exp((double)l[i] - (double)largest) / sum : sigmoid_f64((double)l[i]);
-                    if (bias) c += (double)bias[lane * IPL + i];
-                }
-                key2[i] = key_of(c);
-            }
-            if (sh.groups > 1) keep_groups<double, IPL, L, false>(key2, sh, lane, mine, mine + sh.E);
-            int e2;
-            choose<double, IPL, L, false>(key2, sh, lane, e2);
-            e = e2;
+        for (int i = 0; i < IPL; ++i) {
+            const double r = soft ? scale : reciprocal_wide(1.0 + v[i]);
+            v[i] = soft || l[i] < 0.0f ? v[i] * r : r;
+            if (bias && lane * IPL + i < sh.E) v[i] += (double)bias[lane * IPL + i];
+            if (l[i] == minus_inf) v[i] = -__builtin_inf();
         }
     }
+#pragma unroll
+    for (int i = 0; i < IPL; ++i) v[i] = pack_choice(v[i], lane * IPL + i);
+    bool again = sh.groups > 1 && sh.group_lanes == 0;
+    if (!again) {
+        double *of_group = reinterpret_cast<double *>(mine + sh.E);
+        if (plain) {
+            if (sh.groups > 1) keep_group_lanes<IPL, L, false>(v, sh, lane, of_group);
+            choose<IPL, L, false>(v, sh.k, lane, e);
+        } else {
+            if (sh.groups > 1) again = keep_group_lanes<IPL, L, true>(v, sh, lane, of_group);
+            const unsigned long long close = choose<IPL, L, true>(v, sh.k, lane, e);
+            if (__any(close != 0)) {
+                const float le = e >= 0 ? (float)row[e] : 0.0f, be = e >= 0 && bias ? bias[e] : 0.0f;
+                const float lp = __shfl_up(le, 1, L), bp = __shfl_up(be, 1, L);
+                again |= (close >> lane & 1) && !(le == lp && be == bp);
+            }
+            if (lane >= sh.k) e = -1;
+        }
+    }
+    if (__any(again && live)) e = choose_again<T, IPL, L>(row, live, bias, sh, lane, plain, largest, mine, mine + sh.E);
     // Lane j weighs the j-th choice.
-    const float lj = live && lane < sh.k && e >= 0 ? (float)row[e] : -__builtin_inff();
-    float w;
+    const float lj = live && lane < sh.k && e >= 0 ? (float)row[e] : minus_inf;
     if (sh.renormalise) {
         // Relative to the largest chosen score, so that no sum vanishes: softmax
         // is exp(l) up to a factor; so is the sigmoid, times 1 / (1 + exp(l)).
-        unsigned m = lane < sh.k ? key_of(lj) : 0;
-        const float top = of_key(group_max<L>(m));
-        float p = 0.0f;
-        if (lj != -__builtin_inff()) {
-            p = exp_near(lj - top);
-            if (lj == top) p = 1.0f;  // infinite ones too
-            if (!soft) {
-                // s / sigmoid(top) * (1 + exp(-|top|)) in two ranges, neither of which overflows
-                p = top > 0.0f ? sigmoid_near(lj) : p / (1.0f + exp_near(lj));
-            }
-            if (lj != lj) p = lj;
-        }
+        const float top = of_key(group_max<L>(key_of(lj)));
+        const float p = chosen_share(lj, top, soft);
         const float sum = group_sum<L>(p);
         w = p == 0.0f ? 0.0f : p / sum;
     } else {
-        w = lj == -__builtin_inff() ? 0.0f : (soft ? exp_near(lj - largest) / total : sigmoid_near(lj));
+        w = lj == minus_inf ? 0.0f : (soft ? exp_near(lj - largest) / total : sigmoid_near(lj));
     }
     if (soft && !(largest < __builtin_inff())) w = __builtin_nanf("");  // no softmax over NaN or an infinite score
+    w = e < 0 ? 0.0f : w * sh.scale;
+}
+
+template <typename T, int IPL, int L>
+__global__ __launch_bounds__(kRouteBlock) void route_kernel(const T *__restrict__ scores, const float *__restrict__ bias,
+                                                            RouteShape sh, int *__restrict__ expert,
+                                                            float *__restrict__ weight)
+{
+    extern __shared__ unsigned long long route_lds[];
+    const int lane = threadIdx.x & (L - 1), in_block = threadIdx.x / L;
+    const long long t = (long long)blockIdx.x * (kRouteBlock / L) + in_block;
+    const bool live = t < sh.T;
+    int e;
+    float w;
+    route_token<T, IPL, L>(scores + (live ? t : 0) * sh.E, live, bias, sh, lane, route_lds + in_block * (sh.E + sh.groups),
+                           e, w);
     if (live && lane < sh.k) {
         expert[t * sh.k + lane] = e;
-        weight[t * sh.k + lane] = e < 0 ? 0.0f : w * sh.scale;
+        weight[t * sh.k + lane] = w;
     }
 }
 
@@ -316,8 +463,11 @@ inline int sort_chunk(long long M)
     const long long c = (M + kSortMaxChunks - 1) / kSortMaxChunks;
     return (int)((c < kSortMinChunk ? kSortMinChunk : c) + kSortBlock - 1) / kSortBlock * kSortBlock;
 }
-// wavefronts that count by themselves: as many as fit 64 KB of counters
-inline int sort_waves(int E) { return E < 512 ? kSortWaves : kSortWaves / 2; }
+// wavefronts of a workgroup that count by themselves: as many as fit 64 KB of counters and have slots
+inline int sort_waves(int E, int slots)
+{
+    return std::max(1, std::min(E < 512 ? kSortWaves : kSortWaves / 2, ceil_div(slots, 64)));
+}
 
 __device__ __forceinline__ int id_of(int e, int E) { return (unsigned)e < (unsigned)E ? e : E; }
 
@@ -356,13 +506,13 @@ __device__ __forceinline__ int block_exclusive_sum(int v, int *__restrict__ wave
 // number of slots with a smaller expert, plus those of the same expert in
 // earlier chunks, in earlier wavefronts of the chunk, and in earlier lanes: no
 // order depends on timing.  counts == nullptr: the only chunk there is.
-__global__ __launch_bounds__(kSortBlock) void columns_place_kernel(const int *__restrict__ expert, int M, int E, int chunk,
-                                                                   int chunks, const int *__restrict__ counts, int waves,
-                                                                   int *__restrict__ expert_ptr, int *__restrict__ slot,
-                                                                   int *__restrict__ pos)
+__device__ __forceinline__ void place_chunk(const int *__restrict__ expert, int M, int E, int chunk, int chunks,
+                                            const int *__restrict__ counts, int waves, int *__restrict__ expert_ptr,
+                                            int *__restrict__ slot, int *__restrict__ pos,
+                                            int *__restrict__ place_lds /* waves x (E + 1) */)
 {
-    extern __shared__ int place_lds[];  // waves x (E + 1)
     __shared__ int wave_sum[kSortWaves];
+    __shared__ int part_total[kSortBlock + 1], part_before[kSortBlock + 1];
     const int E1 = E + 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int i = threadIdx.x; i < waves * E1; i += kSortBlock) place_lds[i] = 0;
@@ -375,15 +525,32 @@ __global__ __launch_bounds__(kSortBlock) void columns_place_kernel(const int *__
     int *hist = place_lds + (wave < waves ? wave : 0) * E1;
     for (long long s = first + lane; s < end; s += 64) atomicAdd(&hist[id_of(expert[s], E)], 1);
     __syncthreads();
-    // E1 <= 1025: thread x has expert x, thread 0 the last one too
+    // The other chunks' counts are added up by as many threads as there are, each
+    // a share of the chunks of one expert.
+    const int parts = max(kSortBlock / E1, 1);
+    if (counts) {
+        for (int x = threadIdx.x; x < parts * E1; x += kSortBlock) {
+            const int part = x / E1, e = x - part * E1;
+            int total = 0, before = 0;
+#pragma unroll 8
+            for (int b = part; b < chunks; b += parts) {
+                const int c = counts[(size_t)b * E1 + e];
+                total += c;
+                before += b < (int)blockIdx.x ? c : 0;
+            }
+            part_total[x] = total;
+            part_before[x] = before;
+        }
+        __syncthreads();
+    }
+    // E1 <= 1025: thread x has expert x, the last thread also the 1025th
     int total = 0, before = 0;
     const int e = threadIdx.x;
     if (e < E1) {
         if (counts) {
-            for (int b = 0; b < chunks; ++b) {
-                const int c = counts[(size_t)b * E1 + e];
-                total += c;
-                before += b < (int)blockIdx.x ? c : 0;
+            for (int x = e; x < parts * E1; x += E1) {
+                total += part_total[x];
+                before += part_before[x];
             }
         } else {
             for (int w = 0; w < waves; ++w) total += place_lds[w * E1 + e];
@@ -402,9 +569,7 @@ __global__ __launch_bounds__(kSortBlock) void columns_place_kernel(const int *__
     if (E1 > kSortBlock && threadIdx.x == kSortBlock - 1) {  // E = 1024: the slots without an expert
         const int last = base + total;
         if (blockIdx.x == 0) expert_ptr[E] = last;
-        int at = last;
-        if (counts)
-            for (int b = 0; b < (int)blockIdx.x; ++b) at += counts[(size_t)b * E1 + E];
+        int at = last + (counts ? part_before[E] : 0);
         for (int w = 0; w < waves; ++w) {
             const int c = place_lds[w * E1 + E];
             place_lds[w * E1 + E] = at;
@@ -424,13 +589,9 @@ __global__ __launch_bounds__(kSortBlock) void columns_place_kernel(const int *__
         }
         const int rank = __popcll(same & ((1ull << lane) - 1));
         const int at = in ? hist[id] : 0;
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wave_sync();
         if (in && rank == 0) hist[id] = at + __popcll(same);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wave_sync();
         if (in) {
             slot[at + rank] = (int)s;
             pos[s] = id < E ? at + rank : -1;
@@ -438,12 +599,49 @@ __global__ __launch_bounds__(kSortBlock) void columns_place_kernel(const int *__
     }
 }
 
+__global__ __launch_bounds__(kSortBlock) void columns_place_kernel(const int *__restrict__ expert, int M, int E, int chunk,
+                                                                   int chunks, const int *__restrict__ counts, int waves,
+                                                                   int *__restrict__ expert_ptr, int *__restrict__ slot,
+                                                                   int *__restrict__ pos)
+{
+    extern __shared__ int place_lds[];
+    place_chunk(expert, M, E, chunk, chunks, counts, waves, expert_ptr, slot, pos, place_lds);
+}
+
+// Rows and columns of a few tokens in one launch, where launches are the time:
+// one workgroup routes them all, its choices stay in LDS for the columns.
+template <typename T, int IPL, int L>
+__global__ __launch_bounds__(kSortBlock) void route_few_kernel(const T *__restrict__ scores, const float *__restrict__ bias,
+                                                               RouteShape sh, int *__restrict__ expert,
+                                                               float *__restrict__ weight, int waves,
+                                                               int *__restrict__ expert_ptr, int *__restrict__ slot,
+                                                               int *__restrict__ pos)
+{
+    extern __shared__ unsigned long long route_lds[];
+    __shared__ int ids[kSortBlock / L * (L < MPS_ROUTE_MAX_K ? L : MPS_ROUTE_MAX_K)];
+    const int lane = threadIdx.x & (L - 1), t = threadIdx.x / L;
+    const bool live = t < sh.T;
+    int e = -1;
+    float w = 0.0f;
+    if ((int)(threadIdx.x & ~63u) / L < sh.T)  // wavefronts without a token wait
+        route_token<T, IPL, L>(scores + (size_t)(live ? t : 0) * sh.E, live, bias, sh, lane,
+                               route_lds + min(t, sh.T) * (sh.E + sh.groups), e, w);
+    if (live && lane < sh.k) {
+        expert[t * sh.k + lane] = e;
+        weight[t * sh.k + lane] = w;
+        ids[t * sh.k + lane] = e;
+    }
+    __syncthreads();
+    place_chunk(ids, sh.T * sh.k, sh.E, sh.T * sh.k, 1, nullptr, waves, expert_ptr, slot, pos,
+                reinterpret_cast<int *>(route_lds));
+}
+
 int launch_columns(const int *expert, int M, int E, int *expert_ptr, int *slot, int *pos, void *workspace,
                    hipStream_t st)
 {
     const int chunk = sort_chunk(M);
     const int chunks = M > 0 ? ceil_div(M, chunk) : 1;
-    const int waves = sort_waves(E);
+    const int waves = sort_waves(E, chunk);
     int *counts = chunks > 1 ? static_cast<int *>(workspace) : nullptr;
     if (counts) {
         hipLaunchKernelGGL(columns_count_kernel, dim3(chunks), dim3(kSortBlock), (E + 1) * sizeof(int), st, expert, M, E,
@@ -508,12 +706,7 @@ __global__ __launch_bounds__(kRouteBlock) void route_backward_kernel(const T *__
     float mean = 0.0f;
     if (sh.renormalise) {
         const float top = of_key(group_max<64>(key_of(lj)));
-        float p = 0.0f;
-        if (lj != minus_inf) {
-            p = lj == top ? 1.0f : exp_near(lj - top);
-            if (!soft) p = top > 0.0f ? sigmoid_near(lj) : p / (1.0f + exp_near(lj));
-            if (lj != lj) p = lj;
-        }
+        const float p = chosen_share(lj, top, soft);
         const float sum = group_sum<64>(p);
         const float w = p == 0.0f ? 0.0f : p / sum;
         mean = group_sum<64>(w == 0.0f ? 0.0f : w * g);
@@ -652,24 +845,53 @@ int check_options(const mps_route_options *o, int T, int E, bool choice)
 RouteShape make_shape(const mps_route_options &o, int T, int E)
 {
     const int groups = o.groups > 1 && o.top_groups < o.groups ? o.groups : 1;
-    return RouteShape{T, E, o.k, o.score, groups, E / groups, o.top_groups, o.group_score, o.renormalise, o.scale};
+    return RouteShape{T, E, o.k, o.score, groups, E / groups, o.top_groups, o.group_score, o.renormalise, o.scale, 0};
 }
 
+// Lanes and experts per lane for a token: 16 lanes do four tokens in a wavefront,
+// and their maxima cross lanes in four cheap steps (16384 tokens of 256 experts:
+// ROUTE_LANES); more where the experts or the choices need them.
+template <typename F>
+int with_route_lanes(const RouteShape &sh, F &&f)
+{
+#define MPS_LANES(IPL, L) f(std::integral_constant<int, IPL>{}, std::integral_constant<int, L>{})
+    if (sh.k < 16) {
+        if (sh.E <= 16) return MPS_LANES(1, 16);
+        if (sh.E <= 64) return MPS_LANES(4, 16);
+        if (sh.E <= 128) return MPS_LANES(8, 16);
+        if (sh.E <= 256) return MPS_LANES(16, 16);
+    } else if (sh.k < 32 && sh.E <= 256) {
+        return MPS_LANES(8, 32);
+    }
+    if (sh.k < 32 && sh.E <= 512) return MPS_LANES(16, 32);
+    return MPS_LANES(16, 64);
+#undef MPS_LANES
+}
+
+// `columns`: where rows and columns were made by one launch.
 template <typename T>
-int launch_route(const T *scores, const float *bias, const RouteShape &sh, int *expert, float *weight, hipStream_t st)
+int launch_route(const T *scores, const float *bias, RouteShape sh, int *expert, float *weight, int *expert_ptr,
+                 int *slot, int *pos, bool &columns, hipStream_t st)
 {
     const size_t per_token = (size_t)(sh.groups > 1 ? sh.E + sh.groups : 0) * sizeof(unsigned long long);
-#define MPS_LAUNCH_ROUTE(IPL, L)                                                                                   \
-    hipLaunchKernelGGL((route_kernel<T, IPL, L>), dim3(ceil_div(sh.T, kRouteBlock / L)), dim3(kRouteBlock),        \
-                       per_token * (kRouteBlock / L), st, scores, bias, sh, expert, weight)
-    if (sh.E <= 64) MPS_LAUNCH_ROUTE(1, 64);
-    else if (sh.E <= 128) MPS_LAUNCH_ROUTE(2, 64);
-    else if (sh.E <= 256) MPS_LAUNCH_ROUTE(4, 64);
-    else if (sh.E <= 512) MPS_LAUNCH_ROUTE(8, 64);
-    else MPS_LAUNCH_ROUTE(16, 64);
-#undef MPS_LAUNCH_ROUTE
-    MPS_HIP_TRY(hipGetLastError());
-    return MPS_OK;
+    return with_route_lanes(sh, [&](auto ipl, auto lanes) -> int {
+        constexpr int IPL = decltype(ipl)::value, L = decltype(lanes)::value;
+        if (sh.groups > 1 && sh.group_size % IPL == 0 && (sh.group_size / IPL & (sh.group_size / IPL - 1)) == 0)
+            sh.group_lanes = sh.group_size / IPL;
+        const int waves = sort_waves(sh.E, sh.T * sh.k < 65536 ? sh.T * sh.k : 65536);
+        const size_t few_lds = std::max(per_token * (sh.T + 1), (size_t)waves * (sh.E + 1) * sizeof(int));
+        if (expert_ptr && sh.T <= kSortBlock / L && few_lds <= 64 * 1024 - 16 * 1024) {
+            columns = true;
+            hipLaunchKernelGGL((route_few_kernel<T, IPL, L>), dim3(1), dim3(kSortBlock), few_lds, st, scores, bias, sh,
+                               expert, weight, waves, expert_ptr, slot, pos);
+            MPS_HIP_TRY(hipGetLastError());
+            return MPS_OK;
+        }
+        hipLaunchKernelGGL((route_kernel<T, IPL, L>), dim3(ceil_div(sh.T, kRouteBlock / L)), dim3(kRouteBlock),
+                           per_token * (kRouteBlock / L), st, scores, bias, sh, expert, weight);
+        MPS_HIP_TRY(hipGetLastError());
+        return MPS_OK;
+    });
 }
 
 template <typename T>
@@ -754,13 +976,16 @@ int mps_route(const void *d_scores, int dtype, const float *d_bias, int T, int E
         if (need > 0 && !aligned_to(d_workspace, 16)) return MPS_ERR_ALIGNMENT;
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
+    bool done = false;
     if (T > 0) {
         const RouteShape sh = make_shape(*options, T, E);
-        int r;
-        if (dtype == MPS_F32) r = launch_route(static_cast<const float *>(d_scores), d_bias, sh, d_expert, d_weight, st);
-        else if (dtype == MPS_F16) r = launch_route(static_cast<const half_t *>(d_scores), d_bias, sh, d_expert, d_weight, st);
-        else r = launch_route(static_cast<const bf16_t *>(d_scores), d_bias, sh, d_expert, d_weight, st);
-        if (r != MPS_OK) return r;
+        auto run = [&](auto *scores) {
+            return launch_route(scores, d_bias, sh, d_expert, d_weight, d_expert_ptr, d_slot, d_pos, done, st);
+        };
+        const int r = dtype == MPS_F32   ? run(static_cast<const float *>(d_scores))
+                      : dtype == MPS_F16 ? run(static_cast<const half_t *>(d_scores))
+                                         : run(static_cast<const bf16_t *>(d_scores));
+        if (r != MPS_OK || done) return r;
     }
     return columns ? launch_columns(d_expert, M, E, d_expert_ptr, d_slot, d_pos, d_workspace, st) : MPS_OK;
 }

@@ -31,39 +31,49 @@ class Routing(NamedTuple):
     pos: torch.Tensor
 
 
-def _data(t, name, dims, like=None):
-    """A contiguous matrix of a type that the kernels take; on the device (and of the type) of `like`."""
+def _is(t, dtype, shape, device):
+    """Whether t is a contiguous tensor of this type and shape on GPU number `device`."""
+    return (isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.get_device() == device
+            and device >= 0 and t.is_contiguous())
+
+
+def _first(t, name, dims):
+    """The operand that says of which type and on which device the others are: (type, device)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("%s must be a CUDA/HIP torch tensor" % name)
     if t.dtype not in _DTYPES:
         raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
-    if like is not None and t.dtype != like.dtype:
-        raise TypeError("%s must have dtype %s, got %s" % (name, like.dtype, t.dtype))
-    return _shaped(t, name, dims, like)
+    if t.dim() != dims:
+        raise ValueError("%s must have %d dimensions, got the shape %s" % (name, dims, list(t.shape)))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
+    return t.dtype, t.get_device()
 
 
-def _array(t, name, dtype, dims, like):
+def _need(t, name, dtype, shape, device):
+    if _is(t, dtype, shape, device):
+        return t
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("%s must be a CUDA/HIP torch tensor" % name)
     if t.dtype != dtype:
         raise TypeError("%s must have dtype %s, got %s" % (name, dtype, t.dtype))
-    return _shaped(t, name, dims, like)
-
-
-def _shaped(t, name, dims, like):
-    if t.dim() != len(dims) or any(d is not None and d != s for d, s in zip(dims, t.shape)):
-        raise ValueError("%s must have the shape [%s], got %s"
-                         % (name, ", ".join("any" if d is None else str(d) for d in dims), list(t.shape)))
+    if t.shape != shape:
+        raise ValueError("%s must have the shape %s, got %s" % (name, list(shape), list(t.shape)))
     if not t.is_contiguous():
         raise ValueError("%s must be contiguous" % name)
-    if like is not None and t.device != like.device:
-        raise ValueError("%s is on %s, the other tensors on %s" % (name, t.device, like.device))
-    return t
+    raise ValueError("%s is on %s, the other tensors on cuda:%d" % (name, t.device, device))
+
+
+def _shape_of(t, name, dims):
+    """The shape of a tensor that _need will look at more closely."""
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        raise ValueError("%s must be a tensor of %d dimensions" % (name, dims))
+    return t.shape
 
 
 def _fits(*sizes):
     """Sizes travel as 32-bit ints; a larger one must not come out as another number."""
-    if any(not 0 <= n <= 0x7FFFFFFF for n in sizes):
+    if max(sizes) > 0x7FFFFFFF or min(sizes) < 0:
         check(_cabi.MPS_ERR_UNSUPPORTED, "sizes beyond 32 bits")
 
 
@@ -71,15 +81,16 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _call(name, like, *args):
-    """mps_<name>(args, stream) on the device of `like`."""
+def _call(name, device, *args):
+    """mps_<name>(args, stream) on GPU number `device`, on the stream that is current there."""
     fn = getattr(_cabi.lib(), name)
-    index = like.device.index
-    if index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(index).cuda_stream), name)
+    if device == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
-        with torch.cuda.device(index):
-            check(fn(*args, torch.cuda.current_stream(index).cuda_stream), name)
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        check(status, name)
 
 
 def _options(k, score, groups, top_groups, group_score, renormalise, scale):
@@ -87,15 +98,14 @@ def _options(k, score, groups, top_groups, group_score, renormalise, scale):
         raise ValueError("score must be one of %s" % sorted(_SCORES))
     if group_score not in _GROUP_SCORES:
         raise ValueError("group_score must be one of %s" % sorted(_GROUP_SCORES))
-    return _cabi.RouteOptions(int(k), _SCORES[score], int(groups), int(top_groups), _GROUP_SCORES[group_score],
-                              int(bool(renormalise)), float(scale))
+    return _cabi.RouteOptions(k, _SCORES[score], groups, top_groups, _GROUP_SCORES[group_score], bool(renormalise), scale)
 
 
-def _workspace(T, E, k, like):
+def _workspace(T, E, k, device):
     """Device memory for the columns of a long routing matrix; None where none is needed."""
     need = ctypes.c_size_t()
     check(_cabi.lib().mps_route_workspace_bytes(T, E, k, ctypes.byref(need)), "mps_route_workspace_bytes")
-    ws = torch.empty(need.value, dtype=torch.uint8, device=like.device) if need.value else None
+    ws = torch.empty(need.value, dtype=torch.uint8, device="cuda:%d" % device) if need.value else None
     return ws, need.value
 
 
@@ -108,77 +118,75 @@ def route(scores, k, *, score="softmax", bias=None, groups=1, top_groups=1, grou
     member, or with "top2" as the sum of its two largest); ties go to the lower index, the choice is that of 64 bits.
     Weights are scale * s, with `renormalise` divided by the sum of the chosen s.  A score of -inf is never chosen: a
     slot that finds no expert holds -1, weight 0 and pos -1."""
-    _data(scores, "scores", (None, None))
+    t, device = _first(scores, "scores", 2)
     T, E = scores.shape
     opt = _options(k, score, groups, top_groups, group_score, renormalise, scale)
     if bias is not None:
-        _array(bias, "bias", torch.float32, (E,), scores)
+        _need(bias, "bias", torch.float32, (E,), device)
     if k < 1:
         raise ValueError("k must be positive")
-    _fits(T * k, E)
+    n = T * k
+    _fits(n, E)
+    ws, size = (None, 0) if n <= 2048 else _workspace(T, E, k, device)
     if out is None:
-        ints = torch.empty(3 * T * k + E + 1, dtype=torch.int32, device=scores.device)
-        n = T * k
-        out = Routing(ints[:n].view(T, k), torch.empty((T, k), dtype=torch.float32, device=scores.device), ints[3 * n:],
-                      ints[n:2 * n], ints[2 * n:3 * n].view(T, k))
+        # one allocation: the four arrays of integers, and the weights' bits
+        ints = torch.empty(4 * n + E + 1, dtype=torch.int32, device=scores.device)
+        expert, weight, pos, slot, expert_ptr = ints.split_with_sizes((n, n, n, n, E + 1))
+        out = Routing(expert.view(T, k), weight.view(torch.float32).view(T, k), expert_ptr, slot, pos.view(T, k))
+        at = ints.data_ptr()
+        at = at, at + 4 * n, at + 16 * n, at + 12 * n, at + 8 * n
     else:
-        _check_routing(out, T, E, k, scores)
-    ws, size = _workspace(T, E, k, scores)
-    _call("mps_route", scores, _ptr(scores), _DTYPES[scores.dtype], _ptr(bias), T, E, ctypes.byref(opt),
-          _ptr(out.expert), _ptr(out.weight), _ptr(out.expert_ptr), _ptr(out.slot), _ptr(out.pos), _ptr(ws), size)
+        _need(out.expert, "expert", torch.int32, (T, k), device)
+        _need(out.weight, "weight", torch.float32, (T, k), device)
+        _need(out.expert_ptr, "expert_ptr", torch.int32, (E + 1,), device)
+        _need(out.slot, "slot", torch.int32, (n,), device)
+        _need(out.pos, "pos", torch.int32, (T, k), device)
+        at = tuple(x.data_ptr() for x in out)
+    _call("mps_route", device, scores.data_ptr(), _DTYPES[t], _ptr(bias), T, E, opt, *at, _ptr(ws), size)
     return out
-
-
-def _check_routing(r, T, E, k, like):
-    _array(r.expert, "expert", torch.int32, (T, k), like)
-    _array(r.weight, "weight", torch.float32, (T, k), like)
-    _array(r.expert_ptr, "expert_ptr", torch.int32, (E + 1,), like)
-    _array(r.slot, "slot", torch.int32, (T * k,), like)
-    _array(r.pos, "pos", torch.int32, (T, k), like)
 
 
 def columns(expert, n_experts):
     """(expert_ptr, slot, pos) of a routing matrix whose rows expert int32[T, k] are given (mps_route_columns): a stable
     counting sort.  Ids outside [0, n_experts) count as -1.  With k = 1 and the adapters of the tokens, expert_ptr and
     slot are what adapters_mm takes."""
-    if not isinstance(expert, torch.Tensor) or expert.dim() != 2:
-        raise ValueError("expert must be a matrix [T, k]")
-    T, k = expert.shape
-    _array(expert, "expert", torch.int32, (T, k), expert)
+    T, k = _shape_of(expert, "expert", 2)
+    device = expert.get_device()
+    _need(expert, "expert", torch.int32, (T, k), device)
     _fits(T * k, n_experts)
     ptr = torch.empty(n_experts + 1, dtype=torch.int32, device=expert.device)
     slot = torch.empty(T * k, dtype=torch.int32, device=expert.device)
     pos = torch.empty((T, k), dtype=torch.int32, device=expert.device)
-    ws, size = _workspace(T, n_experts, k, expert)
-    _call("mps_route_columns", expert, _ptr(expert), T, n_experts, k, _ptr(ptr), _ptr(slot), _ptr(pos), _ptr(ws), size)
+    ws, size = _workspace(T, n_experts, k, device)
+    _call("mps_route_columns", device, expert.data_ptr(), T, n_experts, k, ptr.data_ptr(), slot.data_ptr(),
+          pos.data_ptr(), _ptr(ws), size)
     return ptr, slot, pos
 
 
 def route_backward(scores, expert, dweight, *, score="softmax", renormalise=False, scale=1.0, out=None):
     """Gradient of the scores from that of the weights (mps_route_backward)."""
-    _data(scores, "scores", (None, None))
+    t, device = _first(scores, "scores", 2)
     T, E = scores.shape
-    if not isinstance(expert, torch.Tensor) or expert.dim() != 2:
-        raise ValueError("expert must be a matrix [T, k]")
-    k = expert.shape[1]
-    _array(expert, "expert", torch.int32, (T, k), scores)
-    _array(dweight, "dweight", torch.float32, (T, k), scores)
+    k = _shape_of(expert, "expert", 2)[1]
+    _need(expert, "expert", torch.int32, (T, k), device)
+    _need(dweight, "dweight", torch.float32, (T, k), device)
     _fits(T * k, E)
     opt = _options(k, score, 1, 1, "max", renormalise, scale)
-    out = torch.empty_like(scores) if out is None else _data(out, "out", (T, E), scores)
-    _call("mps_route_backward", scores, _ptr(scores), _DTYPES[scores.dtype], _ptr(expert), _ptr(dweight), T, E,
-          ctypes.byref(opt), _ptr(out))
+    out = torch.empty_like(scores) if out is None else _need(out, "out", t, (T, E), device)
+    _call("mps_route_backward", device, scores.data_ptr(), _DTYPES[t], expert.data_ptr(), dweight.data_ptr(), T, E,
+          opt, out.data_ptr())
     return out
 
 
-def _places(slot, k, rows, like, name):
+def _places(slot, k, rows, device):
     """Number of places of rows that are gathered through `slot`, or that stand in order."""
-    _fits(rows * max(k, 1))
     if slot is None:
+        _fits(rows)
         return rows
     if k < 1:
         raise ValueError("k must be positive")
-    _array(slot, "slot", torch.int32, (rows * k,), like)
+    _fits(rows * k)
+    _need(slot, "slot", torch.int32, (rows * k,), device)
     return rows * k
 
 
@@ -187,88 +195,91 @@ def experts_mm(X, W, expert_ptr, *, slot=None, k=1, out=None):
 
     Without `slot` X is [M, K] in the order of the places; with it X holds the tokens, [M / k, K], and row(p) =
     slot[p] // k.  Rows of Y behind expert_ptr[E] are left as they were (undefined in a new tensor)."""
-    _data(X, "X", (None, None))
-    _data(W, "W", (None, None, X.shape[1]), X)
-    E, N, K = W.shape
+    t, device = _first(X, "X", 2)
+    rows, K = X.shape
+    E, N, _ = _shape_of(W, "W", 3)
+    _need(W, "W", t, (E, N, K), device)
+    _need(expert_ptr, "expert_ptr", torch.int32, (E + 1,), device)
+    M = _places(slot, k, rows, device)
     _fits(E, N, K)
-    _array(expert_ptr, "expert_ptr", torch.int32, (E + 1,), X)
-    M = _places(slot, k, X.shape[0], X, "X")
-    out = torch.empty((M, N), dtype=X.dtype, device=X.device) if out is None else _data(out, "out", (M, N), X)
-    _call("mps_experts_mm", X, _ptr(X), _ptr(W), _ptr(out), _DTYPES[X.dtype], _ptr(expert_ptr), _ptr(slot),
-          k if slot is not None else 1, M, E, N, K)
+    out = X.new_empty((M, N)) if out is None else _need(out, "out", t, (M, N), device)
+    _call("mps_experts_mm", device, X.data_ptr(), W.data_ptr(), out.data_ptr(), _DTYPES[t], expert_ptr.data_ptr(),
+          _ptr(slot), k if slot is not None else 1, M, E, N, K)
     return out
 
 
 def experts_mm_dx(dY, W, expert_ptr, *, out=None):
     """Gradient of the rows (mps_experts_mm_dx): dX[p] = dY[p] @ W[e], in the order of the places; that of gathered
     tokens is combine(dX, pos).  Rows behind expert_ptr[E] are left as they were."""
-    _data(dY, "dY", (None, None))
-    _data(W, "W", (None, dY.shape[1], None), dY)
-    E, N, K = W.shape
-    _fits(E, N, K)
-    _array(expert_ptr, "expert_ptr", torch.int32, (E + 1,), dY)
-    M = dY.shape[0]
-    _fits(M)
-    out = torch.empty((M, K), dtype=dY.dtype, device=dY.device) if out is None else _data(out, "out", (M, K), dY)
-    _call("mps_experts_mm_dx", dY, _ptr(dY), _ptr(W), _ptr(out), _DTYPES[dY.dtype], _ptr(expert_ptr), M, E, N, K)
+    t, device = _first(dY, "dY", 2)
+    M, N = dY.shape
+    E, _, K = _shape_of(W, "W", 3)
+    _need(W, "W", t, (E, N, K), device)
+    _need(expert_ptr, "expert_ptr", torch.int32, (E + 1,), device)
+    _fits(M, E, N, K)
+    out = dY.new_empty((M, K)) if out is None else _need(out, "out", t, (M, K), device)
+    _call("mps_experts_mm_dx", device, dY.data_ptr(), W.data_ptr(), out.data_ptr(), _DTYPES[t], expert_ptr.data_ptr(), M,
+          E, N, K)
     return out
+
+
+def _experts_of(expert_ptr):
+    E = _shape_of(expert_ptr, "expert_ptr", 1)[0] - 1
+    if E < 1:
+        raise ValueError("expert_ptr must be an array of E + 1 places")
+    return E
 
 
 def experts_mm_dw(dY, X, expert_ptr, *, slot=None, k=1, out=None):
     """Gradient of the weights (mps_experts_mm_dw): dW[e] = dY[places of e].T @ X[row(places)], zero for an expert
     without places.  `slot` and `k` as in experts_mm."""
-    _data(X, "X", (None, None))
-    M = _places(slot, k, X.shape[0], X, "X")
-    _data(dY, "dY", (M, None), X)
-    E, N, K = _experts_of(expert_ptr), dY.shape[1], X.shape[1]
+    t, device = _first(X, "X", 2)
+    rows, K = X.shape
+    M = _places(slot, k, rows, device)
+    N = _shape_of(dY, "dY", 2)[1]
+    _need(dY, "dY", t, (M, N), device)
+    E = _experts_of(expert_ptr)
+    _need(expert_ptr, "expert_ptr", torch.int32, (E + 1,), device)
     _fits(E, N, K)
-    _array(expert_ptr, "expert_ptr", torch.int32, (E + 1,), X)
-    out = torch.empty((E, N, K), dtype=X.dtype, device=X.device) if out is None else _data(out, "out", (E, N, K), X)
-    _call("mps_experts_mm_dw", X, _ptr(dY), _ptr(X), _ptr(out), _DTYPES[X.dtype], _ptr(expert_ptr), _ptr(slot),
-          k if slot is not None else 1, M, E, N, K)
+    out = X.new_empty((E, N, K)) if out is None else _need(out, "out", t, (E, N, K), device)
+    _call("mps_experts_mm_dw", device, dY.data_ptr(), X.data_ptr(), out.data_ptr(), _DTYPES[t], expert_ptr.data_ptr(),
+          _ptr(slot), k if slot is not None else 1, M, E, N, K)
     return out
-
-
-def _experts_of(expert_ptr):
-    if not isinstance(expert_ptr, torch.Tensor) or expert_ptr.dim() != 1 or expert_ptr.numel() < 2:
-        raise ValueError("expert_ptr must be an array of E + 1 places")
-    return expert_ptr.numel() - 1
 
 
 def combine(Z, pos, weight=None, *, base=None, out=None):
     """Product of the routing matrix with the experts' rows (mps_combine): Y[t] = base[t] + sum_j weight[t, j] *
-    Z[pos[t, j]] over the slots that have a place; weight None = 1."""
-    _data(Z, "Z", (None, None))
+    Z[pos[t, j]] over the slots that have a place; weight None = 1.  `out` may be `base`."""
+    t, device = _first(Z, "Z", 2)
     M, N = Z.shape
-    if not isinstance(pos, torch.Tensor) or pos.dim() != 2:
-        raise ValueError("pos must be a matrix [T, k]")
-    T, k = pos.shape
-    _fits(T * k, M, N)
-    _array(pos, "pos", torch.int32, (T, k), Z)
+    T, k = _shape_of(pos, "pos", 2)
+    _need(pos, "pos", torch.int32, (T, k), device)
     if weight is not None:
-        _array(weight, "weight", torch.float32, (T, k), Z)
+        _need(weight, "weight", torch.float32, (T, k), device)
     if base is not None:
-        _data(base, "base", (T, N), Z)
-    out = torch.empty((T, N), dtype=Z.dtype, device=Z.device) if out is None else _data(out, "out", (T, N), Z)
-    _call("mps_combine", Z, _ptr(Z), _ptr(pos), _ptr(weight), _ptr(base), _ptr(out), _DTYPES[Z.dtype], T, k, M, N)
+        _need(base, "base", t, (T, N), device)
+    _fits(T * k, M, N)
+    out = Z.new_empty((T, N)) if out is None else _need(out, "out", t, (T, N), device)
+    _call("mps_combine", device, Z.data_ptr(), pos.data_ptr(), _ptr(weight), _ptr(base), out.data_ptr(), _DTYPES[t], T, k,
+          M, N)
     return out
 
 
 def combine_backward(dY, Z, weight, expert_ptr, slot):
     """Gradients of combine (mps_combine_backward): {"dZ": [M, N], "dweight": float32[T, k]}; zero where there is no
     expert."""
-    _data(dY, "dY", (None, None))
+    t, device = _first(dY, "dY", 2)
     T, N = dY.shape
-    _array(weight, "weight", torch.float32, (T, None), dY)
-    k = weight.shape[1]
-    _fits(T * k, N)
-    _data(Z, "Z", (T * k, N), dY)
+    k = _shape_of(weight, "weight", 2)[1]
+    _need(weight, "weight", torch.float32, (T, k), device)
+    _need(Z, "Z", t, (T * k, N), device)
     E = _experts_of(expert_ptr)
-    _array(expert_ptr, "expert_ptr", torch.int32, (E + 1,), dY)
-    _array(slot, "slot", torch.int32, (T * k,), dY)
+    _need(expert_ptr, "expert_ptr", torch.int32, (E + 1,), device)
+    _need(slot, "slot", torch.int32, (T * k,), device)
+    _fits(T * k, E, N)
     dZ, dweight = torch.empty_like(Z), torch.empty_like(weight)
-    _call("mps_combine_backward", dY, _ptr(dY), _ptr(Z), _ptr(weight), _ptr(expert_ptr), E, _ptr(slot), _ptr(dZ),
-          _ptr(dweight), _DTYPES[dY.dtype], T, k, N)
+    _call("mps_combine_backward", device, dY.data_ptr(), Z.data_ptr(), weight.data_ptr(), expert_ptr.data_ptr(), E,
+          slot.data_ptr(), dZ.data_ptr(), dweight.data_ptr(), _DTYPES[t], T, k, N)
     return {"dZ": dZ, "dweight": dweight}
 
 
@@ -277,23 +288,25 @@ def adapters_mm(X, A, B, scale, adapter_ptr, row, *, base=None, out=None):
     tokens row[adapter_ptr[a]:adapter_ptr[a + 1]] of adapter a, Y[t] = base[t] for those behind adapter_ptr[E]; A [E, R, K],
     B [E, N, R], scale float32[E] or None.  `row` names every token once (columns() of the tokens' adapters).  `out` may
     be `base`."""
-    _data(X, "X", (None, None))
+    t, device = _first(X, "X", 2)
     T, K = X.shape
-    _data(A, "A", (None, None, K), X)
-    E, R = A.shape[0], A.shape[1]
-    _data(B, "B", (E, None, R), X)
-    N = B.shape[1]
-    _fits(T, E, R, K, N)
+    E, R, _ = _shape_of(A, "A", 3)
+    N = _shape_of(B, "B", 3)[1]
+    _need(A, "A", t, (E, R, K), device)
+    _need(B, "B", t, (E, N, R), device)
     if scale is not None:
-        _array(scale, "scale", torch.float32, (E,), X)
-    _array(adapter_ptr, "adapter_ptr", torch.int32, (E + 1,), X)
-    _array(row, "row", torch.int32, (T,), X)
+        _need(scale, "scale", torch.float32, (E,), device)
+    _need(adapter_ptr, "adapter_ptr", torch.int32, (E + 1,), device)
+    _need(row, "row", torch.int32, (T,), device)
     if base is not None:
-        _data(base, "base", (T, N), X)
-    out = torch.empty((T, N), dtype=X.dtype, device=X.device) if out is None else _data(out, "out", (T, N), X)
+        _need(base, "base", t, (T, N), device)
+    _fits(T, E, R, K, N)
+    out = X.new_empty((T, N)) if out is None else _need(out, "out", t, (T, N), device)
     need = ctypes.c_size_t()
-    check(_cabi.lib().mps_adapters_workspace_bytes(T, E, R, K, ctypes.byref(need)), "mps_adapters_workspace_bytes")
+    status = _cabi.lib().mps_adapters_workspace_bytes(T, E, R, K, ctypes.byref(need))
+    if status:
+        check(status, "mps_adapters_workspace_bytes")
     ws = torch.empty(max(need.value, 16), dtype=torch.uint8, device=X.device)
-    _call("mps_adapters_mm", X, _ptr(X), _ptr(A), _ptr(B), _ptr(scale), _ptr(base), _ptr(out), _DTYPES[X.dtype],
-          _ptr(adapter_ptr), _ptr(row), T, E, R, K, N, _ptr(ws), need.value)
+    _call("mps_adapters_mm", device, X.data_ptr(), A.data_ptr(), B.data_ptr(), _ptr(scale), _ptr(base), out.data_ptr(),
+          _DTYPES[t], adapter_ptr.data_ptr(), row.data_ptr(), T, E, R, K, N, ws.data_ptr(), need.value)
     return out
