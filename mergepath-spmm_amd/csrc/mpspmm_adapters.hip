@@ -11,46 +11,7 @@
 
 namespace {
 
-typedef float float4v __attribute__((ext_vector_type(4)));
-typedef half_t half8v __attribute__((ext_vector_type(8)));
-typedef bf16_t bf16x8v __attribute__((ext_vector_type(8)));
-typedef unsigned uint4v __attribute__((ext_vector_type(4)));
-
 constexpr int kWaves = 4;
-
-template <typename T>
-__device__ __forceinline__ float4v mma(uint4v p, uint4v q, float4v acc)
-{
-    if constexpr (sizeof(T) == 4) {
-        const float4v a = __builtin_bit_cast(float4v, p), b = __builtin_bit_cast(float4v, q);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
-        return acc;
-    } else if constexpr (__is_same(T, half_t)) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, p), __builtin_bit_cast(half8v, q), acc,
-                                                      0, 0, 0);
-    } else {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, p), __builtin_bit_cast(bf16x8v, q),
-                                                       acc, 0, 0, 0);
-    }
-}
-
-// 16 bytes from p, of which `valid` elements exist; zeros for the others.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ uint4v load_chunk(const T *p, int valid)
-{
-    constexpr int V = 16 / sizeof(T);
-    uint4v v = {0, 0, 0, 0};
-    if (valid >= V) {
-        __builtin_memcpy(&v, __builtin_assume_aligned(p, ALIGNED ? 16 : sizeof(T)), 16);
-    } else if (valid > 0) {
-        T part[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) part[i] = i < valid ? p[i] : (T)0.0f;
-        __builtin_memcpy(&v, part, 16);
-    }
-    return v;
-}
 
 struct AdaptersShape {
     int T, E, R, K, N;
@@ -132,8 +93,8 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_shrink_kernel(const T *_
 // it is not rounded to 8 or 11 bits on the way.  fp16 has no room for values
 // from 65520 on: where a tile holds one, all of its V are taken down by 2^16
 // and the sums up again.  RANK: the largest rank, in units of 32.
-// Row g * 4 + d of the b-th matrix instruction is column g * 16 + b * 4 + d, so
-// that a lane ends up with 16 neighbouring columns of a token.
+// Row g * 4 + d of the b-th matrix instruction is the column that leaves a lane
+// with 16 bytes of neighbouring columns, and the four lanes of a token with 64.
 template <typename T, int RANK, int MT, bool ALIGNED>
 __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const float *__restrict__ V,
                                                                       const T *__restrict__ B,
@@ -143,6 +104,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
                                                                       AdaptersShape sh)
 {
     constexpr int C = 16 / sizeof(T), STEP = 4 * C, STEPS = RANK * 32 / STEP, ROWS = 16 * MT;
+    constexpr int PER = C / 4;  // matrix instructions that fill 16 bytes
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i = lane & 15, g = lane >> 4;
     // The tokens without an adapter are one more segment, of which only the base is left.
@@ -212,45 +174,78 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
         }
     }
     const T *b_of = B + (size_t)max(t.expert, 0) * sh.N * sh.R;
-    for (int n0 = blockIdx.x * columns + wave * 64; n0 < min((int)(blockIdx.x + 1) * columns, sh.N); n0 += kWaves * 64) {
+    // Stores are counted with the loads, in order, so that a load behind a store
+    // waits for it: the next 64 columns are asked for before these are stored.
+    // (Ranks over 64 have no registers for two, and one turn.)
+    struct Operands {
+        uint4v p[STEPS][4], y[MT][PER == 1 ? 4 : 2];
+    };
+    auto ask = [&](Operands &o, int n0) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int b = 0; b < 16 / C; ++b) {
+                const int col = n0 + b * 4 * C + g * C;
+                o.y[m][b] = load_chunk<T, ALIGNED>(base + (base && token[m] >= 0 ? (size_t)token[m] * sh.N + col : 0),
+                                                   base && token[m] >= 0 ? sh.N - col : 0);
+            }
+        if (t.expert < 0) return;
+#pragma unroll
+        for (int step = 0; step < STEPS; ++step) {
+            const int r = step * STEP + g * C;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int col = n0 + b / PER * 4 * C + (i >> 2) * C + b % PER * 4 + (i & 3);
+                o.p[step][b] = load_chunk<T, ALIGNED>(b_of + (size_t)(col < sh.N ? col : 0) * sh.R + r,
+                                                      col < sh.N ? sh.R - r : 0);
+            }
+        }
+    };
+    auto finish = [&](const Operands &o, int n0, auto next) {
         float4v acc[MT][4] = {};
         if (t.expert >= 0) {
 #pragma unroll
-            for (int step = 0; step < STEPS; ++step) {
-                if (step * STEP >= sh.R) break;
-                const int r = step * STEP + g * C;
-                uint4v p[4];
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int col = n0 + (i >> 2) * 16 + b * 4 + (i & 3);
-                    p[b] = load_chunk<T, ALIGNED>(b_of + (size_t)(col < sh.N ? col : 0) * sh.R + r, col < sh.N ? sh.R - r : 0);
-                }
+            for (int step = 0; step < STEPS; ++step)
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
-                        acc[m][b] = mma<T>(p[b], high[m][step], acc[m][b]);
-                        if constexpr (sizeof(T) == 2) acc[m][b] = mma<T>(p[b], low[m][step], acc[m][b]);
+                        acc[m][b] = mma<T>(o.p[step][b], high[m][step], acc[m][b]);
+                        if constexpr (sizeof(T) == 2) acc[m][b] = mma<T>(o.p[step][b], low[m][step], acc[m][b]);
                     }
-            }
         }
-        const int col = n0 + g * 16;
+        next();
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            if (token[m] < 0 || col >= sh.N) continue;
-            const size_t at = (size_t)token[m] * sh.N + col;
+            if (token[m] < 0) continue;
             const float up = __is_same(T, half_t) && taken[m] ? 65536.0f : 1.0f;
 #pragma unroll
-            for (int b = 0; b < 16; b += C) {
-                if (col + b >= sh.N) break;
-                float y[C];
+            for (int b = 0; b < 16 / C; ++b) {
+                const int col = n0 + b * 4 * C + g * C;
+                T of_base[C];
+                __builtin_memcpy(of_base, &o.y[m][b], 16);
+                float part[C];
 #pragma unroll
-                for (int c = 0; c < C; ++c) y[c] = 0.0f;
-                if (base) load_vec<T, C, ALIGNED>(y, base + at + b, sh.N - col - b);
-#pragma unroll
-                for (int c = 0; c < C; ++c) y[c] += acc[m][(b + c) / 4][(b + c) % 4] * up;
-                store_vec<T, C, ALIGNED>(Y + at + b, y, sh.N - col - b);
+                for (int c = 0; c < C; ++c)
+                    part[c] = __builtin_fmaf(acc[m][b * PER + c / 4][c % 4], up, (float)of_base[c]);
+                store_vec<T, C, ALIGNED>(Y + (size_t)token[m] * sh.N + col, part, sh.N - col);
             }
+        }
+    };
+    const int end = min((int)(blockIdx.x + 1) * columns, sh.N);
+    int n0 = blockIdx.x * columns + wave * 64;
+    if (n0 >= end) return;
+    Operands now;
+    ask(now, n0);
+    if constexpr (RANK > 2) {
+        finish(now, n0, [] {});
+    } else {
+        for (;; n0 += kWaves * 64) {
+            Operands ahead = now;
+            const int n1 = n0 + kWaves * 64;
+            finish(now, n0, [&] { if (n1 < end) ask(ahead, n1); });
+            if (n1 >= end) break;
+            now = ahead;
         }
     }
 }
@@ -271,9 +266,9 @@ AdaptersShape make_shape(int T, int E, int R, int K, int N)
     return sh;
 }
 
-// MT of the two kernels: what fits the registers beside the rank.
+// MT of the first kernel: what fits the registers beside the rank.  The second is
+// bound by its loads and stores, and takes 16 tokens (MTNOTE).
 constexpr int shrink_tiles(int RT) { return RT <= 4 ? 4 : RT == 8 ? 2 : 1; }
-constexpr int expand_tiles(int RANK) { return RANK <= 2 ? 4 : 1; }
 
 template <typename T, int RT, int MT>
 int launch_shrink(const T *X, const T *A, const int *ptr, const int *row_of, float *V, const AdaptersShape &sh,
@@ -295,7 +290,7 @@ int launch_expand(const float *V, const T *B, const float *scale, const T *base,
     const long long tiles = num_row_tiles(sh.T, sh.E, 16 * MT) + 1;
     // Columns of a workgroup: as many as leave about 1024 of them, at most 1024, so that V is not read too often.
     long long columns = (long long)sh.N * tiles / 1024 / 256 * 256;
-    columns = columns < 256 ? 256 : columns > 1024 ? 1024 : columns;
+    columns = columns < 256 || RANK > 2 ? 256 : columns > 1024 ? 1024 : columns;
     const dim3 grid(ceil_div(sh.N, columns), (unsigned)tiles);
     const bool fast = rows_of_16(B, sh.R, sizeof(T)) && rows_of_16(base, sh.N, sizeof(T)) && rows_of_16(Y, sh.N, sizeof(T));
     if (fast)
@@ -327,8 +322,7 @@ int launch_adapters(const void *X_, const void *A_, const void *B_, const float 
 #undef MPS_SHRINK
     if (rc != MPS_OK) return rc;
 #define MPS_EXPAND(RANK)                                                                                         \
-    return sh.tall ? launch_expand<T, RANK, expand_tiles(RANK)>(V, B, scale, base, Y, ptr, row_of, sh, st)       \
-                   : launch_expand<T, RANK, 1>(V, B, scale, base, Y, ptr, row_of, sh, st)
+    return launch_expand<T, RANK, RANK <= 2 ? 2 : 1>(V, B, scale, base, Y, ptr, row_of, sh, st)
     if (sh.R <= 32) MPS_EXPAND(1);
     if (sh.R <= 64) MPS_EXPAND(2);
     MPS_EXPAND(8);

@@ -20,11 +20,7 @@
 
 namespace {
 
-typedef float float4v __attribute__((ext_vector_type(4)));
-typedef half_t half8v __attribute__((ext_vector_type(8)));
-typedef bf16_t bf16x8v __attribute__((ext_vector_type(8)));
 typedef short short4v __attribute__((ext_vector_type(4)));
-typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v *lds_short4;
 
 constexpr int kTile = 128;
@@ -55,24 +51,6 @@ __device__ __forceinline__ int place_turned(int row, int c)
 {
     if constexpr (sizeof(T) == 2) return (row * 16 + (c ^ (((row & 3) | ((row >> 1) & 4)) << 1))) * 16;
     else return (row * 32 + (c ^ (((row >> 2) & 3) << 2))) * 16;
-}
-
-template <typename T>
-__device__ __forceinline__ float4v mma(uint4v p, uint4v q, float4v acc)
-{
-    if constexpr (sizeof(T) == 4) {
-        // r = 4 g + j of a step is summed by instruction j
-        const float4v a = __builtin_bit_cast(float4v, p), b = __builtin_bit_cast(float4v, q);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
-        return acc;
-    } else if constexpr (__is_same(T, half_t)) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, p), __builtin_bit_cast(half8v, q), acc,
-                                                      0, 0, 0);
-    } else {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, p), __builtin_bit_cast(bf16x8v, q),
-                                                       acc, 0, 0, 0);
-    }
 }
 
 // What a lane feeds to the matrix instruction for 16 neighbouring outer indices,
@@ -109,23 +87,6 @@ __device__ __forceinline__ uint4v fragment(const char *panel, int base, int n, i
         for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const unsigned *>(at + j * 512);
         return v;
     }
-}
-
-// 16 bytes from p, of which `valid` elements exist; zeros for the others.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ uint4v load_chunk(const T *p, int valid)
-{
-    constexpr int V = 16 / sizeof(T);
-    uint4v v = {0, 0, 0, 0};
-    if (valid >= V) {
-        __builtin_memcpy(&v, __builtin_assume_aligned(p, ALIGNED ? 16 : sizeof(T)), 16);
-    } else if (!ALIGNED && valid > 0) {
-        T part[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) part[i] = i < valid ? p[i] : (T)0.0f;
-        __builtin_memcpy(&v, part, 16);
-    }
-    return v;
 }
 
 struct ExpertsShape {
@@ -553,6 +514,92 @@ int launch_stream(const void *A, const void *B, void *out, const int *ptr, const
     return MPS_OK;
 }
 
+// The product where experts have a few rows each, as in decoding: the weights'
+// bytes are the time, and every one is used once.  One workgroup per tile of
+// 16 MT rows and 64 columns; its four wavefronts take 128 bytes of the rows in
+// turn, straight into the matrix instructions' registers, and add up through
+// LDS.  No barrier until the end, so that many loads are on their way.
+constexpr int kFewWaves = 4, kFewColumns = 4;  // in 16s
+
+template <typename T, int MT, bool ALIGNED>
+__global__ __launch_bounds__(64 * kFewWaves) void experts_few_kernel(const T *__restrict__ X, const T *__restrict__ W,
+                                                                     T *__restrict__ Y, const int *__restrict__ ptr,
+                                                                     const int *__restrict__ slot, ExpertsShape sh)
+{
+    constexpr int C = 16 / sizeof(T), STEP = 4 * C, RT = kFewColumns;
+    __shared__ float4v join[kFewWaves][RT][64];
+    const RowTile t = find_row_tile<16 * MT>(ptr, sh.E, sh.M, blockIdx.x / sh.col_tiles);
+    if (t.rows == 0) return;
+    const int col0 = blockIdx.x % sh.col_tiles * (16 * RT);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int i = lane & 15, g = lane >> 4;
+    const T *x[MT], *w[RT];
+    bool live[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        int from = 16 * m + i < t.rows ? t.first + 16 * m + i : -1;
+        if (slot && from >= 0) {
+            const int s = slot[from];
+            from = (unsigned)s < (unsigned)sh.M ? (int)token_of(s, sh) : -1;
+        }
+        live[m] = from >= 0;
+        x[m] = X + (size_t)max(from, 0) * sh.K;
+    }
+#pragma unroll
+    for (int n = 0; n < RT; ++n) w[n] = W + ((size_t)t.expert * sh.N + min(col0 + n * 16 + i, sh.N - 1)) * sh.K;
+    float4v acc[MT][RT] = {};
+    for (int base = wave * 2 * STEP; base < sh.K; base += kFewWaves * 2 * STEP) {
+        uint4v p[2][RT], q[2][MT];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int k = base + half * STEP + g * C;
+#pragma unroll
+            for (int n = 0; n < RT; ++n) p[half][n] = load_chunk<T, ALIGNED>(w[n] + k, sh.K - k);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) q[half][m] = load_chunk<T, ALIGNED>(x[m] + k, live[m] ? sh.K - k : 0);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < RT; ++n) acc[m][n] = mma<T>(p[half][n], q[half][m], acc[m][n]);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        if (m > 0) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < RT; ++n) join[wave][n][lane] = acc[m][n];
+        __syncthreads();
+        const int col = col0 + wave * 16 + g * 4;  // as many 16s of columns as wavefronts
+        if (16 * m + i < t.rows && col < sh.N) {
+            float4v sum = join[0][wave][lane];
+#pragma unroll
+            for (int other = 1; other < kFewWaves; ++other) sum += join[other][wave][lane];
+            const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+            store_vec<T, 4, ALIGNED>(Y + (size_t)(t.first + 16 * m + i) * sh.N + col, v, sh.N - col);
+        }
+    }
+}
+static_assert(kFewColumns == kFewWaves, "a wavefront adds up 16 columns");
+
+template <typename T, int MT>
+int launch_few(const void *X, const void *W, void *Y, const int *ptr, const int *slot, ExpertsShape sh, bool fast,
+               hipStream_t st)
+{
+    sh.col_tiles = ceil_div(sh.N, 16 * kFewColumns);
+    const long long blocks = num_row_tiles(sh.M, sh.E, 16 * MT) * sh.col_tiles;
+    if (blocks > INT_MAX) return MPS_ERR_UNSUPPORTED;
+#define MPS_LAUNCH_FEW(ALIGNED)                                                                                       \
+    hipLaunchKernelGGL((experts_few_kernel<T, MT, ALIGNED>), dim3((unsigned)blocks), dim3(64 * kFewWaves), 0, st,     \
+                       static_cast<const T *>(X), static_cast<const T *>(W), static_cast<T *>(Y), ptr, slot, sh)
+    if (fast) MPS_LAUNCH_FEW(true);
+    else MPS_LAUNCH_FEW(false);
+#undef MPS_LAUNCH_FEW
+    MPS_HIP_TRY(hipGetLastError());
+    return MPS_OK;
+}
+
 template <typename T, Product WHAT>
 int launch_experts(const void *A, const void *B, void *out, const int *ptr, const int *slot, int k, int M, int E, int N,
                    int K, hipStream_t st)
@@ -567,6 +614,11 @@ int launch_experts(const void *A, const void *B, void *out, const int *ptr, cons
     // every operand's rows are N or K long
     const bool fast = rows_of_16(A, WHAT == kForward ? K : N, sizeof(T)) && rows_of_16(B, K, sizeof(T)) &&
                       rows_of_16(out, WHAT == kForward ? N : K, sizeof(T));
+    if constexpr (WHAT == kForward) {
+        // Few rows an expert (32 tokens, 6 of 64 experts, 2048 x 1024 bf16: FEW_TIME).
+        if (M <= 8LL * E) return launch_few<T, 1>(A, B, out, ptr, slot, sh, fast, st);
+        if (M <= 24LL * E) return launch_few<T, 2>(A, B, out, ptr, slot, sh, fast, st);
+    }
     // offsets of 32 bits inside X or dY and inside the matrix of an expert
     const long long far = INT_MAX / (long long)sizeof(T);
     const bool near = (long long)M * (WHAT == kForward ? K : N) <= far && (long long)N * K <= far &&

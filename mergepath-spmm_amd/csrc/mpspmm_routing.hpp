@@ -75,6 +75,49 @@ __device__ __forceinline__ void store_vec(T *p, const float (&v)[V], int valid)
     }
 }
 
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef half_t half8v __attribute__((ext_vector_type(8)));
+typedef bf16_t bf16x8v __attribute__((ext_vector_type(8)));
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+
+// acc += p q^T for 16 rows p and q of one matrix step, 16 bytes of the summed
+// index in every lane: lane l holds row l % 16, chunk l / 16.  The result: lane l
+// holds q = l % 16 and four neighbouring p from (l / 16) * 4 on.
+template <typename T>
+__device__ __forceinline__ float4v mma(uint4v p, uint4v q, float4v acc)
+{
+    if constexpr (sizeof(T) == 4) {
+        // instruction j sums element j of every chunk
+        const float4v a = __builtin_bit_cast(float4v, p), b = __builtin_bit_cast(float4v, q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
+        return acc;
+    } else if constexpr (__is_same(T, half_t)) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, p), __builtin_bit_cast(half8v, q), acc,
+                                                      0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, p), __builtin_bit_cast(bf16x8v, q),
+                                                       acc, 0, 0, 0);
+    }
+}
+
+// 16 bytes from p, of which `valid` elements exist; zeros for the others.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ uint4v load_chunk(const T *p, int valid)
+{
+    constexpr int V = 16 / sizeof(T);
+    uint4v v = {0, 0, 0, 0};
+    if (valid >= V) {
+        __builtin_memcpy(&v, __builtin_assume_aligned(p, ALIGNED ? 16 : sizeof(T)), 16);
+    } else if (valid > 0) {
+        T part[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) part[i] = i < valid ? p[i] : (T)0.0f;
+        __builtin_memcpy(&v, part, 16);
+    }
+    return v;
+}
+
 // ---------------------------------------------------------------------------
 // Segments.  ptr[0 .. E] cuts the places 0 .. M - 1 into the experts' runs.
 // Values are clamped so that no caller's table reaches outside the arrays.
