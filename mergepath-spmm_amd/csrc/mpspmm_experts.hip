@@ -1,12 +1,12 @@
 // Products of the experts: a matrix for every expert, times the rows that the
 // routing matrix sends there, with their two gradients.
 //
-// One tile kernel does all three.  A workgroup owns a 128 x 128 tile of the
-// result: P counts its columns (contiguous in memory), Q its rows,
+// One scheme does all three.  A workgroup owns a tile of the result, of panels
+// of S = 128 or 64: P counts its columns (contiguous in memory), Q its rows,
 //   D[q, p] = sum_r Q[q, r] P[p, r],
 // with r the summed index.  An operand is stored either with r contiguous
 // (rows of 128 bytes of r are staged, one per q or p) or with p / q contiguous
-// (rows of 128 elements are staged, one per r, and turned while they are read
+// (rows of S elements are staged, one per r, and turned while they are read
 // from LDS):
 //                r             P                       Q
 //   product      K             W[e], r contiguous      X, r contiguous
@@ -23,16 +23,13 @@ namespace {
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v *lds_short4;
 
-constexpr int kTile = 128;
 constexpr int kThreads = 256;
-constexpr int kChunks = kTile * 128 / 16 / kThreads;  // 16-byte chunks of an operand's stage per thread: 4
 
 template <typename T>
 struct Elem {
     static constexpr int kPerChunk = 16 / sizeof(T);
     static constexpr int kDepth = 128 / sizeof(T);      // r per stage
     static constexpr int kStep = 4 * kPerChunk;         // r per matrix step: lane group g takes chunk g
-    static constexpr int kRowChunks = kTile / kPerChunk;  // chunks of a staged row of 128 elements
 };
 
 // Where chunk c of staged row `row` lies, so that the 16 lanes that read
@@ -43,48 +40,51 @@ __device__ __forceinline__ int place_rows(int row, int c)
 {
     return (row * 8 + (c ^ ((row >> 1) & 7))) * 16;
 }
-//   p / q contiguous, 16-bit: 16 chunks a row, the turning read takes 32 bytes
-//   of each of the rows 8 g + 0 .. 3 (or 4 .. 7), g = 0 .. 3; fp32: 32 chunks a
-//   row, lanes take 64 bytes of the rows 4 g + j.
-template <typename T>
+//   p / q contiguous, 16-bit: the turning read takes 32 bytes of each of the rows
+//   8 g + 0 .. 3 (or 4 .. 7), g = 0 .. 3; fp32: lanes take 64 bytes of the rows
+//   4 g + j.
+template <typename T, int S>
 __device__ __forceinline__ int place_turned(int row, int c)
 {
-    if constexpr (sizeof(T) == 2) return (row * 16 + (c ^ (((row & 3) | ((row >> 1) & 4)) << 1))) * 16;
-    else return (row * 32 + (c ^ (((row >> 2) & 3) << 2))) * 16;
+    constexpr int CHUNKS = S / Elem<T>::kPerChunk;  // of a staged row
+    if constexpr (sizeof(T) == 4) return (row * CHUNKS + (c ^ (((row >> 2) & 3) << 2))) * 16;
+    else if constexpr (S == 128) return (row * CHUNKS + (c ^ (((row & 3) | ((row >> 1) & 4)) << 1))) * 16;
+    else return (row * CHUNKS + (c ^ (((row >> 1 & 1) | ((row >> 2) & 2)) << 1))) * 16;
 }
 
 // What a lane feeds to the matrix instruction for 16 neighbouring outer indices,
 // the (first + n)-th 16 of a panel, and matrix step s.  The places above differ
 // between n and s by sums and exclusive ors of constants only, so that a lane
 // needs one base: `first` a multiple of a power of two above n.
-template <typename T, bool TURNED>
+template <typename T, bool TURNED, int S>
 __device__ __forceinline__ int fragment_base(int first, int lane)
 {
     const int i = lane & 15, g = lane >> 4;
     if constexpr (!TURNED) return place_rows<T>(first * 16 + i, g);
-    else if constexpr (sizeof(T) == 2) return place_turned<T>(8 * g + (i >> 2), first * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
-    else return place_turned<T>(4 * g, first * 4 + (i >> 2)) + (i & 3) * 4;
+    else if constexpr (sizeof(T) == 2) return place_turned<T, S>(8 * g + (i >> 2), first * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
+    else return place_turned<T, S>(4 * g, first * 4 + (i >> 2)) + (i & 3) * 4;
 }
-template <typename T, bool TURNED>
+template <typename T, bool TURNED, int S>
 __device__ __forceinline__ uint4v fragment(const char *panel, int base, int n, int s)
 {
+    constexpr int ROW_BYTES = S * sizeof(T);  // of a staged row to be turned
     if constexpr (!TURNED) {
         return *reinterpret_cast<const uint4v *>(panel + (base ^ (s << 6)) + n * 2048);
     } else if constexpr (sizeof(T) == 2) {
         // 16 lanes read a block of 4 rows (r) by 16 elements, 8 bytes each, and get it turned
-        const char *at = panel + (base ^ (n << 5)) + s * 8192;
+        const char *at = panel + (base ^ (n << 5)) + s * (32 * ROW_BYTES);
         union {
             short4v part[2];
             uint4v all;
         } u;
         u.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)at);
-        u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)(at + 1024));
+        u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)(at + 4 * ROW_BYTES));
         return u.all;
     } else {
-        const char *at = panel + (base ^ (n << 6)) + s * 8192;
+        const char *at = panel + (base ^ (n << 6)) + s * (16 * ROW_BYTES);
         uint4v v;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const unsigned *>(at + j * 512);
+        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const unsigned *>(at + j * ROW_BYTES);
         return v;
     }
 }
@@ -111,31 +111,33 @@ __device__ __forceinline__ unsigned token_of(unsigned slot, const ExpertsShape &
 
 enum Product { kForward, kRows, kWeights };
 
-template <typename T, Product WHAT, bool ALIGNED>
+template <typename T, Product WHAT, int S, bool ALIGNED>
 __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__restrict__ A, const T *__restrict__ B,
                                                                    T *__restrict__ out, const int *__restrict__ ptr,
                                                                    const int *__restrict__ slot, ExpertsShape sh)
 {
     // product: A = X, B = W, out = Y; dX: A = dY, B = W, out = dX; dW: A = dY, B = X, out = dW
     constexpr bool PT = WHAT != kForward, QT = WHAT == kWeights;
-    constexpr int V = Elem<T>::kPerChunk, DEPTH = Elem<T>::kDepth;
-    __shared__ __attribute__((aligned(16))) char stage_p[2][kTile * 128];
-    __shared__ __attribute__((aligned(16))) char stage_q[2][kTile * 128];
+    constexpr int V = Elem<T>::kPerChunk, DEPTH = Elem<T>::kDepth, ROW = S / V;
+    constexpr int CHUNKS = S * 128 / 16 / kThreads;  // 16-byte chunks of an operand's stage per thread
+    constexpr int F = S / 32;                        // 16s of a wavefront's share, either way
+    __shared__ __attribute__((aligned(16))) char stage_p[2][S * 128];
+    __shared__ __attribute__((aligned(16))) char stage_q[2][S * 128];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int cols = WHAT == kForward ? sh.N : sh.K;
     const int number = xcd_tile(blockIdx.x, gridDim.x);
-    const int col0 = number % sh.col_tiles * kTile;
+    const int col0 = number % sh.col_tiles * S;
     const int rest = number / sh.col_tiles;
     int expert, row0, rows, first, depth;  // rows of the tile in the result; places summed over from `first` on
     if constexpr (WHAT == kWeights) {
         expert = rest / sh.row_tiles;
-        row0 = rest % sh.row_tiles * kTile;
-        rows = min(sh.N - row0, kTile);
+        row0 = rest % sh.row_tiles * S;
+        rows = min(sh.N - row0, S);
         first = clamp_place(ptr[expert], sh.M);
         depth = max(clamp_place(ptr[expert + 1], sh.M) - first, 0);
     } else {
-        const RowTile t = find_row_tile<kTile>(ptr, sh.E, sh.M, rest);
+        const RowTile t = find_row_tile<S>(ptr, sh.E, sh.M, rest);
         if (t.rows == 0) return;
         expert = t.expert;
         row0 = first = t.first;
@@ -145,13 +147,13 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
     const T *W = WHAT == kWeights ? nullptr : B + (size_t)expert * sh.N * sh.K;
 
     // The chunks that this thread stages.
-    const T *p_src[kChunks], *q_src[kChunks];
-    int p_valid[kChunks], q_valid[kChunks];  // turned: elements from the chunk's column on; else unused (row given or null)
+    const T *p_src[CHUNKS], *q_src[CHUNKS];
+    int p_valid[CHUNKS], q_valid[CHUNKS];  // turned: elements from the chunk's column on; else unused (row given or null)
 #pragma unroll
-    for (int n = 0; n < kChunks; ++n) {
+    for (int n = 0; n < CHUNKS; ++n) {
         const int id = tid + n * kThreads;
         if constexpr (PT) {
-            const int c = id % Elem<T>::kRowChunks;
+            const int c = id % ROW;
             p_src[n] = (WHAT == kRows ? W : B) + col0 + c * V;
             p_valid[n] = cols - (col0 + c * V);
         } else {
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
             p_src[n] = col0 + row < cols ? W + (size_t)(col0 + row) * sh.K : nullptr;
         }
         if constexpr (QT) {
-            const int c = id % Elem<T>::kRowChunks;
+            const int c = id % ROW;
             q_src[n] = A + row0 + c * V;
             q_valid[n] = sh.N - (row0 + c * V);
         } else {
@@ -175,13 +177,13 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
             }
         }
     }
-    uint4v p_hold[kChunks], q_hold[kChunks];
+    uint4v p_hold[CHUNKS], q_hold[CHUNKS];
     auto fetch = [&](int r0) {
 #pragma unroll
-        for (int n = 0; n < kChunks; ++n) {
+        for (int n = 0; n < CHUNKS; ++n) {
             const int id = tid + n * kThreads;
             if constexpr (PT) {
-                const int r = r0 + id / Elem<T>::kRowChunks;
+                const int r = r0 + id / ROW;
                 long long from = -1;
                 if (r < depth) {
                     from = r;
@@ -199,7 +201,7 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
                 p_hold[n] = load_chunk<T, ALIGNED>(p_src[n] + r, p_src[n] ? depth - r : 0);
             }
             if constexpr (QT) {
-                const int r = r0 + id / Elem<T>::kRowChunks;
+                const int r = r0 + id / ROW;
                 q_hold[n] = load_chunk<T, ALIGNED>(q_src[n] + (size_t)(first + (r < depth ? r : 0)) * sh.N,
                                                    r < depth ? q_valid[n] : 0);
             } else {
@@ -210,20 +212,20 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
     };
     auto put = [&](int buffer) {
 #pragma unroll
-        for (int n = 0; n < kChunks; ++n) {
+        for (int n = 0; n < CHUNKS; ++n) {
             const int id = tid + n * kThreads;
-            const int p_at = PT ? place_turned<T>(id / Elem<T>::kRowChunks, id % Elem<T>::kRowChunks)
+            const int p_at = PT ? place_turned<T, S>(id / ROW, id % ROW)
                                 : place_rows<T>(id / 8, id % 8);
-            const int q_at = QT ? place_turned<T>(id / Elem<T>::kRowChunks, id % Elem<T>::kRowChunks)
+            const int q_at = QT ? place_turned<T, S>(id / ROW, id % ROW)
                                 : place_rows<T>(id / 8, id % 8);
             *reinterpret_cast<uint4v *>(stage_p[buffer] + p_at) = p_hold[n];
             *reinterpret_cast<uint4v *>(stage_q[buffer] + q_at) = q_hold[n];
         }
     };
 
-    float4v acc[4][4] = {};  // [q][p]
-    const int p_base = (wave & 1) * 64, q_base = (wave >> 1) * 64;
-    const int p_at = fragment_base<T, PT>(p_base / 16, lane), q_at = fragment_base<T, QT>(q_base / 16, lane);
+    float4v acc[F][F] = {};  // [q][p]
+    const int p_base = (wave & 1) * (S / 2), q_base = (wave >> 1) * (S / 2);
+    const int p_at = fragment_base<T, PT, S>(p_base / 16, lane), q_at = fragment_base<T, QT, S>(q_base / 16, lane);
     if (depth > 0) {
         fetch(0);
         put(0);
@@ -235,16 +237,16 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
         if (more) fetch(r0 + DEPTH);
 #pragma unroll
         for (int s = 0; s < DEPTH / Elem<T>::kStep; ++s) {
-            uint4v p[4], q[4];
+            uint4v p[F], q[F];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                p[n] = fragment<T, PT>(stage_p[buffer], p_at, n, s);
-                q[n] = fragment<T, QT>(stage_q[buffer], q_at, n, s);
+            for (int n = 0; n < F; ++n) {
+                p[n] = fragment<T, PT, S>(stage_p[buffer], p_at, n, s);
+                q[n] = fragment<T, QT, S>(stage_q[buffer], q_at, n, s);
             }
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
+            for (int a = 0; a < F; ++a)
 #pragma unroll
-                for (int b = 0; b < 4; ++b) acc[a][b] = mma<T>(p[b], q[a], acc[a][b]);
+                for (int b = 0; b < F; ++b) acc[a][b] = mma<T>(p[b], q[a], acc[a][b]);
         }
         if (more) put(buffer ^ 1);
         __syncthreads();
@@ -253,13 +255,13 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
 
     // Lane: q = lane % 16, four p from (lane / 16) * 4 on.
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
+    for (int a = 0; a < F; ++a) {
         const int q = q_base + 16 * a + (lane & 15);
         if (q >= rows) continue;
         T *row = out + (WHAT == kWeights ? (size_t)expert * sh.N * sh.K + (size_t)(row0 + q) * sh.K
                                          : (size_t)(row0 + q) * cols);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < F; ++b) {
             const int p = col0 + p_base + 16 * b + (lane >> 4) * 4;
             const float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
             if (p < cols) store_vec<T, 4, ALIGNED>(row + p, v, cols - p);
@@ -270,19 +272,19 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
 // The same products where rows are whole 16 bytes.  The stages come straight
 // from memory into LDS, two of them in turn: while the matrix instructions work
 // on one, the other is on its way.
-//   PP, QP  panels of 128 in the tile's columns and rows
+//   PP, QP  panels of S in the tile's columns and rows
 //   WP, WQ  wavefronts that share them
 typedef __attribute__((address_space(3))) void *lds_ptr;
 
-template <typename T, Product WHAT, int PP, int QP, int WP, int WQ>
+template <typename T, Product WHAT, int S, int PP, int QP, int WP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T *__restrict__ A, const T *__restrict__ B,
                                                                          T *__restrict__ out,
                                                                          const int *__restrict__ ptr,
                                                                          const int *__restrict__ slot, ExpertsShape sh)
 {
     constexpr bool PT = WHAT != kForward, QT = WHAT == kWeights;
-    constexpr int V = Elem<T>::kPerChunk, DEPTH = Elem<T>::kDepth, ROW = Elem<T>::kRowChunks;
-    constexpr int THREADS = 64 * WP * WQ, BP = PP * kTile, BQ = QP * kTile, PANEL = kTile * 128;
+    constexpr int V = Elem<T>::kPerChunk, DEPTH = Elem<T>::kDepth, ROW = S / V;
+    constexpr int THREADS = 64 * WP * WQ, BP = PP * S, BQ = QP * S, PANEL = S * 128;
     constexpr int PC = PP * PANEL / 16 / THREADS, QC = QP * PANEL / 16 / THREADS;  // chunks of a thread
     constexpr int FP = BP / 16 / WP, FQ = BQ / 16 / WQ;                           // fragments of a wavefront
     __shared__ __attribute__((aligned(16))) char stage0[(PP + QP) * PANEL];
@@ -323,7 +325,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     const long long q_step = (QT ? (long long)DEPTH * sh.N : DEPTH) * (long long)sizeof(T);
     constexpr bool LIST = WHAT == kWeights;  // rows of P are looked up for every stage
     // where chunk n begins in its staged row, and the summed index it begins with in a stage
-    auto turned_at = [&](int n) { return place_turned<T>(tid / ROW + n * THREADS / ROW % DEPTH, tid % ROW) / 16 % ROW * V; };
+    auto turned_at = [&](int n) { return place_turned<T, S>(tid / ROW + n * THREADS / ROW % DEPTH, tid % ROW) / 16 % ROW * V; };
     const int row_at = place_rows<T>(tid / 8, tid % 8) / 16 % 8 * V;  // the same for all n
     static_assert(THREADS / 8 % 16 == 0, "rows of equal place");
     auto p_r = [&](int n) { return PT ? tid / ROW + n * THREADS / ROW % DEPTH : row_at; };
@@ -332,7 +334,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     for (int n = 0; n < PC; ++n) {
         const int panel = n * THREADS / (PANEL / 16);
         if constexpr (PT) {
-            const int col = min(col0 + panel * kTile + turned_at(n), cols - V);
+            const int col = min(col0 + panel * S + turned_at(n), cols - V);
             p_off[n] = (unsigned)((LIST ? 0u : (unsigned)p_r(n) * (unsigned)sh.K) + col) * (unsigned)sizeof(T);
         } else {
             const int col = min(col0 + (n * THREADS + tid) / 8, cols - 1);
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     for (int n = 0; n < QC; ++n) {
         const int panel = n * THREADS / (PANEL / 16);
         if constexpr (QT) {
-            const int at = min(row0 + panel * kTile + turned_at(n), sh.N - V);
+            const int at = min(row0 + panel * S + turned_at(n), sh.N - V);
             q_off[n] = ((unsigned)q_r(n) * (unsigned)sh.N + at) * (unsigned)sizeof(T);
         } else {
             const int at = min((n * THREADS + tid) / 8, rows - 1);
@@ -408,9 +410,9 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     const int q_part = EIGHT ? (wave >> 1 & 1) | (wave >> 2) << 1 : wave / WP;
     const int p_base = p_part * (FP * 16), q_base = q_part * (FQ * 16);
     const bool busy = q_base < rows && col0 + p_base < cols;
-    static_assert(FP <= 8 && FQ <= 8, "a wavefront's part of an operand lies in one panel");
-    const int p_at = p_base / kTile * PANEL + fragment_base<T, PT>(p_base % kTile / 16, lane);
-    const int q_at = (PP + q_base / kTile) * PANEL + fragment_base<T, QT>(q_base % kTile / 16, lane);
+    static_assert(FP * 16 <= S && FQ * 16 <= S, "a wavefront's part of an operand lies in one panel");
+    const int p_at = p_base / S * PANEL + fragment_base<T, PT, S>(p_base % S / 16, lane);
+    const int q_at = (PP + q_base / S) * PANEL + fragment_base<T, QT, S>(q_base % S / 16, lane);
     auto arrive = [] {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): own chunks have come, own reads of LDS are done
@@ -427,11 +429,11 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     uint4v q[2][FQ], p[2][HALF];
     auto read_q = [&](const char *stage, int s, int to) {
 #pragma unroll
-        for (int n = 0; n < FQ; ++n) q[to][n] = fragment<T, QT>(stage, q_at, n, s);
+        for (int n = 0; n < FQ; ++n) q[to][n] = fragment<T, QT, S>(stage, q_at, n, s);
     };
     auto read_p = [&](const char *stage, int s, int half) {
 #pragma unroll
-        for (int n = 0; n < HALF; ++n) p[half][n] = fragment<T, PT>(stage, p_at, half * HALF + n, s);
+        for (int n = 0; n < HALF; ++n) p[half][n] = fragment<T, PT, S>(stage, p_at, half * HALF + n, s);
     };
     auto group = [&](int of, int half) {
         __builtin_amdgcn_sched_barrier(0);
@@ -500,14 +502,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     }
 }
 
-template <typename T, Product WHAT, int PP, int QP, int WP, int WQ>
+template <typename T, Product WHAT, int S, int PP, int QP, int WP, int WQ>
 int launch_stream(const void *A, const void *B, void *out, const int *ptr, const int *slot, ExpertsShape sh, hipStream_t st)
 {
-    sh.col_tiles = ceil_div(WHAT == kForward ? sh.N : sh.K, PP * kTile);
-    sh.row_tiles = ceil_div(sh.N, QP * kTile);
-    const long long others = WHAT == kWeights ? (long long)sh.E * sh.row_tiles : num_row_tiles(sh.M, sh.E, QP * kTile);
+    sh.col_tiles = ceil_div(WHAT == kForward ? sh.N : sh.K, PP * S);
+    sh.row_tiles = ceil_div(sh.N, QP * S);
+    const long long others = WHAT == kWeights ? (long long)sh.E * sh.row_tiles : num_row_tiles(sh.M, sh.E, QP * S);
     if (others * sh.col_tiles > INT_MAX) return MPS_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((experts_stream_kernel<T, WHAT, PP, QP, WP, WQ>), dim3((unsigned)(others * sh.col_tiles)),
+    hipLaunchKernelGGL((experts_stream_kernel<T, WHAT, S, PP, QP, WP, WQ>), dim3((unsigned)(others * sh.col_tiles)),
                        dim3(64 * WP * WQ), 0, st, static_cast<const T *>(A), static_cast<const T *>(B),
                        static_cast<T *>(out), ptr, slot, sh);
     MPS_HIP_TRY(hipGetLastError());
@@ -600,17 +602,31 @@ int launch_few(const void *X, const void *W, void *Y, const int *ptr, const int 
     return MPS_OK;
 }
 
+template <typename T, Product WHAT, int S>
+int launch_tile(const void *A, const void *B, void *out, const int *ptr, const int *slot, ExpertsShape sh, bool fast,
+                hipStream_t st)
+{
+    sh.col_tiles = ceil_div(WHAT == kForward ? sh.N : sh.K, S);
+    sh.row_tiles = ceil_div(sh.N, S);
+    const long long others = WHAT == kWeights ? (long long)sh.E * sh.row_tiles : num_row_tiles(sh.M, sh.E, S);
+    if (others * sh.col_tiles > INT_MAX) return MPS_ERR_UNSUPPORTED;
+#define MPS_LAUNCH_TILE(ALIGNED)                                                                                 \
+    hipLaunchKernelGGL((experts_tile_kernel<T, WHAT, S, ALIGNED>), dim3((unsigned)(others * sh.col_tiles)),      \
+                       dim3(kThreads), 0, st, static_cast<const T *>(A), static_cast<const T *>(B),              \
+                       static_cast<T *>(out), ptr, slot, sh)
+    if (fast) MPS_LAUNCH_TILE(true);
+    else MPS_LAUNCH_TILE(false);
+#undef MPS_LAUNCH_TILE
+    MPS_HIP_TRY(hipGetLastError());
+    return MPS_OK;
+}
+
 template <typename T, Product WHAT>
 int launch_experts(const void *A, const void *B, void *out, const int *ptr, const int *slot, int k, int M, int E, int N,
                    int K, hipStream_t st)
 {
     ExpertsShape sh{M, E, N, K, k, 0, 0, 0, 0};
     divide_by(k, sh.k_magic, sh.k_shift);
-    sh.col_tiles = ceil_div(WHAT == kForward ? N : K, kTile);
-    sh.row_tiles = ceil_div(N, kTile);
-    const long long others = WHAT == kWeights ? (long long)E * sh.row_tiles : num_row_tiles(M, E, kTile);
-    if (others * sh.col_tiles > INT_MAX) return MPS_ERR_UNSUPPORTED;
-    const unsigned grid = (unsigned)(others * sh.col_tiles);
     // every operand's rows are N or K long
     const bool fast = rows_of_16(A, WHAT == kForward ? K : N, sizeof(T)) && rows_of_16(B, K, sizeof(T)) &&
                       rows_of_16(out, WHAT == kForward ? N : K, sizeof(T));
@@ -619,26 +635,24 @@ int launch_experts(const void *A, const void *B, void *out, const int *ptr, cons
         if (M <= 8LL * E) return launch_few<T, 1>(A, B, out, ptr, slot, sh, fast, st);
         if (M <= 24LL * E) return launch_few<T, 2>(A, B, out, ptr, slot, sh, fast, st);
     }
+    // Tiles of 64 where tiles of 128 would leave compute units without one.
+    const long long tiles = WHAT == kWeights ? (long long)E * ceil_div(N, 128) * ceil_div(K, 128)
+                                             : ((long long)M / 128 + (E < M ? E : M)) * ceil_div(WHAT == kForward ? N : K, 128);
+    const bool small = tiles < 512;
     // offsets of 32 bits inside X or dY and inside the matrix of an expert
     const long long far = INT_MAX / (long long)sizeof(T);
     const bool near = (long long)M * (WHAT == kForward ? K : N) <= far && (long long)N * K <= far &&
                       (WHAT != kWeights || (long long)M * K <= far);
     if (fast && near) {
         if constexpr (sizeof(T) == 2 && WHAT != kWeights) {
-            if ((long long)M >= 384LL * E) return launch_stream<T, WHAT, 2, 2, 2, 4>(A, B, out, ptr, slot, sh, st);
+            if ((long long)M >= 384LL * E) return launch_stream<T, WHAT, 128, 2, 2, 2, 4>(A, B, out, ptr, slot, sh, st);
         }
-        return launch_stream<T, WHAT, 1, 1, 2, 2>(A, B, out, ptr, slot, sh, st);
+        return small ? launch_stream<T, WHAT, 64, 1, 1, 2, 2>(A, B, out, ptr, slot, sh, st)
+                     : launch_stream<T, WHAT, 128, 1, 1, 2, 2>(A, B, out, ptr, slot, sh, st);
     }
-#define MPS_LAUNCH_EXPERTS(ALIGNED)                                                                              \
-    hipLaunchKernelGGL((experts_tile_kernel<T, WHAT, ALIGNED>), dim3(grid), dim3(kThreads), 0, st,               \
-                       static_cast<const T *>(A), static_cast<const T *>(B), static_cast<T *>(out), ptr, slot, sh)
-    if (fast) MPS_LAUNCH_EXPERTS(true);
-    else MPS_LAUNCH_EXPERTS(false);
-#undef MPS_LAUNCH_EXPERTS
-    MPS_HIP_TRY(hipGetLastError());
-    return MPS_OK;
+    return small ? launch_tile<T, WHAT, 64>(A, B, out, ptr, slot, sh, fast, st)
+                 : launch_tile<T, WHAT, 128>(A, B, out, ptr, slot, sh, fast, st);
 }
-
 template <Product WHAT>
 int experts_entry(const void *A, const void *B, void *out, int dtype, const int *ptr, const int *slot, int k, int M,
                   int E, int N, int K, void *stream)

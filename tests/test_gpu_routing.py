@@ -374,6 +374,58 @@ def test_experts_unaligned(r, dev, t):
     assert torch.equal(r.experts_mm_dw(shifted(dY), shifted(X), ptr.to(dev)), r.experts_mm_dw(dY.to(dev), X.to(dev), ptr.to(dev)))
 
 
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("counts,N,K", [([30 + e % 7 for e in range(130)], 520, 72), ([30 + e % 7 for e in range(130)], 515, 67),
+                                        ([500, 0, 390, 640], 304, 136), ([500, 0, 390, 640], 301, 131)])
+def test_experts_many_tiles(r, dev, t, counts, N, K):
+    """Enough tiles, and long enough segments, for the larger tile shapes, with rows of whole 16 bytes and others."""
+    t = TYPES[t]
+    ptr, M = segments(counts)
+    X, W, dY = normal(1, M, K, t=t), normal(2, len(counts), N, K, t=t, scale=K ** -0.5), normal(3, M, N, t=t)
+    x, w, dy, p = X.to(dev), W.to(dev), dY.to(dev), ptr.to(dev)
+    Y, dX, dW = r.experts_mm(x, w, p), r.experts_mm_dx(dy, w, p), r.experts_mm_dw(dy, x, p)
+    X, W, dY = X.double(), W.double(), dY.double()
+    for e in range(len(counts)):
+        a = slice(int(ptr[e]), int(ptr[e + 1]))
+        if counts[e]:
+            close(Y[a], X[a] @ W[e].t(), X[a].abs() @ W[e].abs().t(), K, t)
+            close(dX[a], dY[a] @ W[e], dY[a].abs() @ W[e].abs(), N, t)
+        close(dW[e], dY[a].t() @ X[a], dY[a].abs().t() @ X[a].abs(), counts[e], t)
+
+
+def test_experts_offsets_beyond_32_bits(r, dev):
+    """Rows and weights that lie further than 2^32 bytes from where their matrices begin."""
+    t = torch.bfloat16
+    K, N, M = 4096, 16, (1 << 19) + 40  # X: 4.3 GB
+    ptr = torch.tensor([0, M - 30, M], dtype=torch.int32)
+    X = torch.zeros(M, K, dtype=t, device=dev)
+    tail = normal(1, 64, K, t=t)
+    X[-64:] = tail.to(dev)
+    W = normal(2, 2, N, K, t=t, scale=K ** -0.5)
+    Y = r.experts_mm(X, W.to(dev), ptr.to(dev))[-64:]
+    for rows, e in ((slice(0, 34), 0), (slice(34, 64), 1)):
+        x, w = tail[rows].double(), W[e].double()
+        close(Y[rows], x @ w.t(), x.abs() @ w.abs().t(), K, t)
+    dY = torch.zeros(M, N, dtype=t, device=dev)
+    dY[-64:] = normal(3, 64, N, t=t).to(dev)
+    d = dY[-64:].cpu().double()
+    dW = r.experts_mm_dw(dY, X, ptr.to(dev))
+    close(dW[1], d[34:].t() @ tail[34:].double(), d[34:].abs().t() @ tail[34:].double().abs(), 30, t)
+    # the matrix [M, K] as dX, written to its end
+    dX = r.experts_mm_dx(dY, W.to(dev), ptr.to(dev), out=X)[-64:]
+    close(dX[34:], d[34:] @ W[1].double(), d[34:].abs() @ W[1].double().abs(), N, t)
+    del X, dX
+    N = K = 16384
+    W = torch.zeros(9, N, K, dtype=t, device=dev)  # 4.8 GB
+    W[8, -32:] = normal(4, 32, K, t=t, scale=K ** -0.5).to(dev)
+    x = normal(5, 40, K, t=t)
+    for counts in ([0] * 8 + [40], [4] * 8 + [8]):
+        ptr, M = segments(counts)
+        Y = r.experts_mm(x.to(dev), W, ptr.to(dev))
+        a, w = x[-counts[8]:].double(), W[8, -32:].cpu().double()
+        close(Y[-counts[8]:, -32:], a @ w.t(), a.abs() @ w.abs().t(), K, t)
+
+
 def test_experts_infinities_stay_in_their_rows(r, dev):
     """Infinities and NaN in one row, or in rows that no expert has, reach no other row."""
     ptr, M = segments([3, 2], 3)
