@@ -157,18 +157,6 @@ __device__ __forceinline__ double min_f64(double a, double b)
     asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
     return r;
 }
-template <int L>
-__device__ __forceinline__ double group_max_f64(double v)
-{
-    if constexpr (L > 1) v = max_f64(v, lane_partner_f64<1>(v));
-    if constexpr (L > 2) v = max_f64(v, lane_partner_f64<2>(v));
-    if constexpr (L > 4) v = max_f64(v, lane_partner_f64<4>(v));
-    if constexpr (L > 8) v = max_f64(v, lane_partner_f64<8>(v));
-    if constexpr (L > 16) v = max_f64(v, lane_partner_f64<16>(v));
-    if constexpr (L > 32) v = max_f64(v, lane_partner_f64<32>(v));
-    return v;
-}
-
 // How near two packed choice scores may be and still not be told apart: a score
 // is off by 2^-44 of one at most, the tag by 2^-42 of the whole.
 __device__ __forceinline__ double doubt(double a, double b)
@@ -194,7 +182,7 @@ __device__ __forceinline__ unsigned long long choose(double (&v)[IPL], int k, in
         for (int step = 1; step < IPL; step *= 2)
 #pragma unroll
             for (int i = 0; i + step < IPL; i += 2 * step) m[i] = max_f64(m[i], m[i + step]);
-        const double best = group_max_f64<L>(m[0]);
+        const double best = fold_group<L>(m[0], max_f64);
         const bool is = high_word(best) != kNeverChosen;
         if constexpr (WATCH) {
             if (j > 0 && is && last - best <= doubt(last, best)) close |= 1ull << j;
@@ -221,13 +209,13 @@ __device__ __forceinline__ bool keep_group_lanes(double (&v)[IPL], const RouteSh
         second = max_f64(second, min_f64(first, v[i]));
         first = max_f64(first, v[i]);
     }
-#define MPS_MERGE_STEP(STEP)                                                                        \
-    if constexpr (L > STEP) {                                                                       \
-        if (sh.group_lanes > STEP) {                                                                \
-            const double f = lane_partner_f64<STEP>(first), g = lane_partner_f64<STEP>(second);     \
-            second = max_f64(min_f64(first, f), max_f64(second, g));                                \
-            first = max_f64(first, f);                                                              \
-        }                                                                                           \
+#define MPS_MERGE_STEP(STEP)                                                                              \
+    if constexpr (L > STEP) {                                                                             \
+        if (sh.group_lanes > STEP) {                                                                      \
+            const double low = fold<STEP>(first, min_f64);                                                \
+            second = max_f64(low, fold<STEP>(second, max_f64));                                           \
+            first = fold<STEP>(first, max_f64);                                                           \
+        }                                                                                                 \
     }
     MPS_MERGE_STEP(1) MPS_MERGE_STEP(2) MPS_MERGE_STEP(4) MPS_MERGE_STEP(8) MPS_MERGE_STEP(16) MPS_MERGE_STEP(32)
 #undef MPS_MERGE_STEP
@@ -608,9 +596,12 @@ __global__ __launch_bounds__(kSortBlock) void columns_place_kernel(const int *__
     place_chunk(expert, M, E, chunk, chunks, counts, waves, expert_ptr, slot, pos, place_lds);
 }
 
-// Rows and columns of a few tokens in one launch, where launches are the time:
-// one workgroup routes them all, its choices stay in LDS for the columns.
-template <typename T, int IPL, int L>
+// Rows and columns of a few tokens in one launch, where launches and latency are
+// the time: one workgroup, a wavefront for every token in turn, so that a lane
+// has few experts; the choices stay in LDS for the columns.
+constexpr int kFewTokens = 16;
+
+template <typename T, int IPL>
 __global__ __launch_bounds__(kSortBlock) void route_few_kernel(const T *__restrict__ scores, const float *__restrict__ bias,
                                                                RouteShape sh, int *__restrict__ expert,
                                                                float *__restrict__ weight, int waves,
@@ -618,23 +609,23 @@ __global__ __launch_bounds__(kSortBlock) void route_few_kernel(const T *__restri
                                                                int *__restrict__ pos)
 {
     extern __shared__ unsigned long long route_lds[];
-    __shared__ int ids[kSortBlock / L * (L < MPS_ROUTE_MAX_K ? L : MPS_ROUTE_MAX_K)];
-    const int lane = threadIdx.x & (L - 1), t = threadIdx.x / L;
-    const bool live = t < sh.T;
-    int e = -1;
-    float w = 0.0f;
-    if ((int)(threadIdx.x & ~63u) / L < sh.T)  // wavefronts without a token wait
-        route_token<T, IPL, L>(scores + (size_t)(live ? t : 0) * sh.E, live, bias, sh, lane,
-                               route_lds + min(t, sh.T) * (sh.E + sh.groups), e, w);
-    if (live && lane < sh.k) {
-        expert[t * sh.k + lane] = e;
-        weight[t * sh.k + lane] = w;
-        ids[t * sh.k + lane] = e;
+    __shared__ int ids[kFewTokens * MPS_ROUTE_MAX_K];
+    const int lane = threadIdx.x & 63, t = threadIdx.x >> 6;
+    if (t < sh.T) {
+        int e;
+        float w;
+        route_token<T, IPL, 64>(scores + (size_t)t * sh.E, true, bias, sh, lane, route_lds + t * (sh.E + sh.groups), e, w);
+        if (lane < sh.k) {
+            expert[t * sh.k + lane] = e;
+            weight[t * sh.k + lane] = w;
+            ids[t * sh.k + lane] = e;
+        }
     }
     __syncthreads();
     place_chunk(ids, sh.T * sh.k, sh.E, sh.T * sh.k, 1, nullptr, waves, expert_ptr, slot, pos,
                 reinterpret_cast<int *>(route_lds));
 }
+static_assert(kFewTokens <= kSortWaves, "a wavefront for every token");
 
 int launch_columns(const int *expert, int M, int E, int *expert_ptr, int *slot, int *pos, void *workspace,
                    hipStream_t st)
@@ -727,8 +718,8 @@ __global__ __launch_bounds__(kRouteBlock) void route_backward_kernel(const T *__
             d = l == minus_inf ? 0.0f : -(exp_near(l - largest) / total) * (sh.scale * mean);
         }
         for (int j = 0; j < sh.k; ++j) {
-            const int ej = __shfl(e, j, 64);
-            const float pj = __shfl(part, j, 64);
+            const int ej = __builtin_amdgcn_readlane(e, j);
+            const float pj = bits_float(__builtin_amdgcn_readlane(float_bits(part), j));
             if (ej == i) d += pj;
         }
         if (i < sh.E) out[i] = (T)d;
@@ -802,23 +793,28 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T *__restri
     const T *y_row = dY + (long long)(routed ? s / k : 0) * N;
     const T *z_row = Z + (long long)p * N;
     T *out = dZ + (long long)p * N;
+    // A load behind a store waits for it, so that several chunks of both rows are
+    // loaded before any is stored.
+    constexpr int U = 4;
     float dot = 0.0f;
-    for (int col = lane * V; col < N; col += 64 * V) {
-        float y[V], z[V];
-        if (routed) {
-            load_vec<T, V, ALIGNED>(y, y_row + col, N - col);
-            if (dweight) {
-                load_vec<T, V, ALIGNED>(z, z_row + col, N - col);
+    for (int first = lane * V; first < N; first += U * 64 * V) {
+        float y[U][V], z[U][V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) dot = __builtin_fmaf(y[i], z[i], dot);
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) y[i] *= w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) y[i] = 0.0f;
+        for (int u = 0; u < U; ++u) {
+            const int col = first + u * 64 * V;
+            load_vec<T, V, ALIGNED>(y[u], y_row + col, routed ? N - col : 0);
+            load_vec<T, V, ALIGNED>(z[u], z_row + col, routed && dweight ? N - col : 0);
         }
-        store_vec<T, V, ALIGNED>(out + col, y, N - col);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int col = first + u * 64 * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                dot = __builtin_fmaf(y[u][i], z[u][i], dot);
+                y[u][i] = routed ? y[u][i] * w : 0.0f;
+            }
+            if (col < N) store_vec<T, V, ALIGNED>(out + col, y[u], N - col);
+        }
     }
     if (dweight && known) {
         dot = group_sum<64>(dot);
@@ -874,19 +870,28 @@ int launch_route(const T *scores, const float *bias, RouteShape sh, int *expert,
                  int *slot, int *pos, bool &columns, hipStream_t st)
 {
     const size_t per_token = (size_t)(sh.groups > 1 ? sh.E + sh.groups : 0) * sizeof(unsigned long long);
+    auto fit_groups = [&](int ipl) {
+        const int lanes = sh.group_size / ipl;
+        sh.group_lanes = sh.groups > 1 && sh.group_size % ipl == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+    };
+    if (expert_ptr && sh.T <= (sh.E <= 256 ? kFewTokens : kFewTokens / 4)) {
+        const int waves = sort_waves(sh.E, sh.T * sh.k);
+        const size_t lds = std::max(per_token * (sh.T + 1), (size_t)waves * (sh.E + 1) * sizeof(int));
+        columns = true;
+#define MPS_LAUNCH_FEW(IPL)                                                                                         \
+    fit_groups(IPL);                                                                                                \
+    hipLaunchKernelGGL((route_few_kernel<T, IPL>), dim3(1), dim3(kSortBlock), lds, st, scores, bias, sh, expert,    \
+                       weight, waves, expert_ptr, slot, pos)
+        if (sh.E <= 64) { MPS_LAUNCH_FEW(1); }
+        else if (sh.E <= 256) { MPS_LAUNCH_FEW(4); }
+        else { MPS_LAUNCH_FEW(16); }
+#undef MPS_LAUNCH_FEW
+        MPS_HIP_TRY(hipGetLastError());
+        return MPS_OK;
+    }
     return with_route_lanes(sh, [&](auto ipl, auto lanes) -> int {
         constexpr int IPL = decltype(ipl)::value, L = decltype(lanes)::value;
-        if (sh.groups > 1 && sh.group_size % IPL == 0 && (sh.group_size / IPL & (sh.group_size / IPL - 1)) == 0)
-            sh.group_lanes = sh.group_size / IPL;
-        const int waves = sort_waves(sh.E, sh.T * sh.k < 65536 ? sh.T * sh.k : 65536);
-        const size_t few_lds = std::max(per_token * (sh.T + 1), (size_t)waves * (sh.E + 1) * sizeof(int));
-        if (expert_ptr && sh.T <= kSortBlock / L && few_lds <= 64 * 1024 - 16 * 1024) {
-            columns = true;
-            hipLaunchKernelGGL((route_few_kernel<T, IPL, L>), dim3(1), dim3(kSortBlock), few_lds, st, scores, bias, sh,
-                               expert, weight, waves, expert_ptr, slot, pos);
-            MPS_HIP_TRY(hipGetLastError());
-            return MPS_OK;
-        }
+        fit_groups(IPL);
         hipLaunchKernelGGL((route_kernel<T, IPL, L>), dim3(ceil_div(sh.T, kRouteBlock / L)), dim3(kRouteBlock),
                            per_token * (kRouteBlock / L), st, scores, bias, sh, expert, weight);
         MPS_HIP_TRY(hipGetLastError());

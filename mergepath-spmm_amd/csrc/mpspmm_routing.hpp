@@ -176,71 +176,58 @@ __device__ __forceinline__ unsigned dpp(unsigned v)
 {
     return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
 }
-template <int STEP>
-__device__ __forceinline__ unsigned lane_partner(unsigned v)
+// op(own value, that of the lane STEP further round), within 8 and 16 lanes by
+// moving data between lanes; across 16 and 32 by exchanging rows of lanes
+// between two copies, which leaves the two values side by side.  The lanes
+// below STEP agree already, so the mirrored halves do for 4 and 8.
+template <int STEP, typename V, typename F>
+__device__ __forceinline__ V fold(V v, F op)
 {
-    if constexpr (STEP == 1) return dpp<0xB1>(v);         // quad_perm 1,0,3,2
-    else if constexpr (STEP == 2) return dpp<0x4E>(v);    // quad_perm 2,3,0,1
-    else if constexpr (STEP == 4) return dpp<0x141>(v);   // the other half of 8 lanes (quads agree already)
-    else if constexpr (STEP == 8) return dpp<0x140>(v);   // the other half of 16 lanes
-    else return (unsigned)__shfl_xor((int)v, STEP, 64);
+    static_assert(sizeof(V) == 4 || sizeof(V) == 8, "one or two registers");
+    constexpr int WORDS = sizeof(V) / 4;
+    unsigned own[WORDS], other[WORDS];
+    __builtin_memcpy(own, &v, sizeof(V));
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+        if constexpr (STEP == 1) other[i] = dpp<0xB1>(own[i]);        // quad_perm 1,0,3,2
+        else if constexpr (STEP == 2) other[i] = dpp<0x4E>(own[i]);   // quad_perm 2,3,0,1
+        else if constexpr (STEP == 4) other[i] = dpp<0x141>(own[i]);  // mirrored within 8 lanes
+        else if constexpr (STEP == 8) other[i] = dpp<0x140>(own[i]);  // mirrored within 16 lanes
+        else {
+            const auto both = STEP == 16 ? __builtin_amdgcn_permlane16_swap(own[i], own[i], false, false)
+                                         : __builtin_amdgcn_permlane32_swap(own[i], own[i], false, false);
+            own[i] = both[0];
+            other[i] = both[1];
+        }
+    }
+    V a, b;
+    __builtin_memcpy(&a, own, sizeof(V));
+    __builtin_memcpy(&b, other, sizeof(V));
+    return op(a, b);
 }
-template <int L>
-__device__ __forceinline__ unsigned group_max(unsigned v)
+template <int L, typename V, typename F>
+__device__ __forceinline__ V fold_group(V v, F op)
 {
-    if constexpr (L > 1) v = max(v, lane_partner<1>(v));
-    if constexpr (L > 2) v = max(v, lane_partner<2>(v));
-    if constexpr (L > 4) v = max(v, lane_partner<4>(v));
-    if constexpr (L > 8) v = max(v, lane_partner<8>(v));
-    if constexpr (L > 16) v = max(v, lane_partner<16>(v));
-    if constexpr (L > 32) v = max(v, lane_partner<32>(v));
+    if constexpr (L > 1) v = fold<1>(v, op);
+    if constexpr (L > 2) v = fold<2>(v, op);
+    if constexpr (L > 4) v = fold<4>(v, op);
+    if constexpr (L > 8) v = fold<8>(v, op);
+    if constexpr (L > 16) v = fold<16>(v, op);
+    if constexpr (L > 32) v = fold<32>(v, op);
     return v;
 }
-template <int STEP>
-__device__ __forceinline__ unsigned long long lane_partner64(unsigned long long v)
+template <int L, typename V>
+__device__ __forceinline__ V group_max(V v)
 {
-    return ((unsigned long long)lane_partner<STEP>((unsigned)(v >> 32)) << 32) | lane_partner<STEP>((unsigned)v);
+    return fold_group<L>(v, [](V a, V b) { return max(a, b); });
 }
-template <int L>
-__device__ __forceinline__ unsigned long long group_max(unsigned long long v)
+template <int L, typename V>
+__device__ __forceinline__ V group_sum(V v)
 {
-    if constexpr (L > 1) v = max(v, lane_partner64<1>(v));
-    if constexpr (L > 2) v = max(v, lane_partner64<2>(v));
-    if constexpr (L > 4) v = max(v, lane_partner64<4>(v));
-    if constexpr (L > 8) v = max(v, lane_partner64<8>(v));
-    if constexpr (L > 16) v = max(v, lane_partner64<16>(v));
-    if constexpr (L > 32) v = max(v, lane_partner64<32>(v));
-    return v;
+    return fold_group<L>(v, [](V a, V b) { return a + b; });
 }
 __device__ __forceinline__ float bits_float(unsigned u) { return __builtin_bit_cast(float, u); }
 __device__ __forceinline__ unsigned float_bits(float f) { return __builtin_bit_cast(unsigned, f); }
-template <int L>
-__device__ __forceinline__ float group_sum(float v)
-{
-    if constexpr (L > 1) v += bits_float(lane_partner<1>(float_bits(v)));
-    if constexpr (L > 2) v += bits_float(lane_partner<2>(float_bits(v)));
-    if constexpr (L > 4) v += bits_float(lane_partner<4>(float_bits(v)));
-    if constexpr (L > 8) v += bits_float(lane_partner<8>(float_bits(v)));
-    if constexpr (L > 16) v += bits_float(lane_partner<16>(float_bits(v)));
-    if constexpr (L > 32) v += bits_float(lane_partner<32>(float_bits(v)));
-    return v;
-}
-template <int STEP>
-__device__ __forceinline__ double lane_partner_f64(double v)
-{
-    return __builtin_bit_cast(double, lane_partner64<STEP>(__builtin_bit_cast(unsigned long long, v)));
-}
-template <int L>
-__device__ __forceinline__ double group_sum(double v)
-{
-    if constexpr (L > 1) v += lane_partner_f64<1>(v);
-    if constexpr (L > 2) v += lane_partner_f64<2>(v);
-    if constexpr (L > 4) v += lane_partner_f64<4>(v);
-    if constexpr (L > 8) v += lane_partner_f64<8>(v);
-    if constexpr (L > 16) v += lane_partner_f64<16>(v);
-    if constexpr (L > 32) v += lane_partner_f64<32>(v);
-    return v;
-}
 
 }  // namespace
 

@@ -9,6 +9,7 @@ tensors as `out` arguments where the caller wants to own them.  Calls run on the
 which need not be the current device.  No counterpart in the reference.
 """
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -93,12 +94,15 @@ def _call(name, device, *args):
         check(status, name)
 
 
+@functools.lru_cache(maxsize=64)
 def _options(k, score, groups, top_groups, group_score, renormalise, scale):
+    """mps_route_options, as an argument of a call.  The structure is only read."""
     if score not in _SCORES:
         raise ValueError("score must be one of %s" % sorted(_SCORES))
     if group_score not in _GROUP_SCORES:
         raise ValueError("group_score must be one of %s" % sorted(_GROUP_SCORES))
-    return _cabi.RouteOptions(k, _SCORES[score], groups, top_groups, _GROUP_SCORES[group_score], bool(renormalise), scale)
+    return ctypes.byref(_cabi.RouteOptions(k, _SCORES[score], groups, top_groups, _GROUP_SCORES[group_score],
+                                           bool(renormalise), scale))
 
 
 def _workspace(T, E, k, device):
