@@ -409,10 +409,13 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     const int p_part = EIGHT ? (wave & 1) ^ (wave >> 2) : wave % WP;
     const int q_part = EIGHT ? (wave >> 1 & 1) | (wave >> 2) << 1 : wave / WP;
     const int p_base = p_part * (FP * 16), q_base = q_part * (FQ * 16);
+    // Two loops, one of requests alone: branches within one make the compiler wait
+    // for what is on its way to LDS.  dW has the branches (with two loops it has
+    // not the registers: 436 us in place of 245, 32768 rows 1024 x 2048 bf16).
     const bool busy = q_base < rows && col0 + p_base < cols;
     static_assert(FP * 16 <= S && FQ * 16 <= S, "a wavefront's part of an operand lies in one panel");
-    const int p_at = p_base / S * PANEL + fragment_base<T, PT, S>(p_base % S / 16, lane);
-    const int q_at = (PP + q_base / S) * PANEL + fragment_base<T, QT, S>(q_base % S / 16, lane);
+    int p_at = p_base / S * PANEL + fragment_base<T, PT, S>(p_base % S / 16, lane);
+    int q_at = (PP + q_base / S) * PANEL + fragment_base<T, QT, S>(q_base % S / 16, lane);
     auto arrive = [] {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): own chunks have come, own reads of LDS are done
@@ -444,8 +447,11 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
         __builtin_amdgcn_sched_barrier(0);
     };
     auto turn = [&](auto works, char *now, const char *next, int r0) {
-        constexpr bool busy = decltype(works)::value;
-        if constexpr (busy) {
+        const bool on = LIST ? busy : decltype(works)::value;
+        // the places that follow from these are made anew in every turn, not kept in registers for all
+        if constexpr (PT) asm volatile("" : "+v"(p_at));
+        if constexpr (QT) asm volatile("" : "+v"(q_at));
+        if (on) {
             read_p(now, 0, 1);
             group(0, 0);
             read_q(now, 1, 1);
@@ -455,14 +461,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
             group(1, 0);
         }
         arrive();  // the next stage has come, and everybody is done with this one
-        if constexpr (busy) {
+        if (on) {
             read_q(next, 0, 0);
             read_p(next, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         issue(now, r0 + 2 * DEPTH);
         if constexpr (LIST) look_up(r0 + 3 * DEPTH);
-        if constexpr (busy) group(1, 1);
+        if (on) group(1, 1);
     };
 
     // Two stages a turn, behind the end of the sum ones of zeros.
@@ -472,7 +478,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
     arrive();
     issue(stage1, DEPTH);
     if constexpr (LIST) look_up(2 * DEPTH);
-    if (busy) {
+    if (LIST || busy) {
         read_q(stage0, 0, 0);
         read_p(stage0, 0, 0);
         for (int r0 = 0; r0 < depth; r0 += 2 * DEPTH) {
@@ -644,7 +650,7 @@ int launch_experts(const void *A, const void *B, void *out, const int *ptr, cons
     const bool near = (long long)M * (WHAT == kForward ? K : N) <= far && (long long)N * K <= far &&
                       (WHAT != kWeights || (long long)M * K <= far);
     if (fast && near) {
-        if constexpr (sizeof(T) == 2 && WHAT != kWeights) {
+        if constexpr (sizeof(T) == 2) {
             if ((long long)M >= 384LL * E) return launch_stream<T, WHAT, 128, 2, 2, 2, 4>(A, B, out, ptr, slot, sh, st);
         }
         return small ? launch_stream<T, WHAT, 64, 1, 1, 2, 2>(A, B, out, ptr, slot, sh, st)
