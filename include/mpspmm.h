@@ -738,9 +738,11 @@ int mps_combine_backward(const void *d_dY, const void *d_Z, const float *d_weigh
  * matrix with k = 1):
  *   d_Y[t, :] = d_base[t, :] + d_scale[a] * (d_X[t, :] * d_A[a]^T) * d_B[a]^T
  * and d_Y[t, :] = d_base[t, :] for the tokens behind d_adapter_ptr[E].
- * d_base NULL = 0 and may be d_Y; d_scale NULL = 1.  R <= 256.  Every token
- * has to be in d_row once.  Workspace: mps_adapters_workspace_bytes. */
+ * d_base NULL = 0 and may be d_Y; d_scale NULL = 1.  R <= 256, E <= 1024 and
+ * T <= MPS_ADAPTERS_MAX_TOKENS, else MPS_ERR_UNSUPPORTED.  Every token has to
+ * be in d_row once.  Workspace: mps_adapters_workspace_bytes. */
 #define MPS_ADAPTERS_MAX_RANK 256
+#define MPS_ADAPTERS_MAX_TOKENS 524280
 int mps_adapters_workspace_bytes(int T, int E, int R, int K, size_t *bytes_out);
 int mps_adapters_mm(const void *d_X, const void *d_A, const void *d_B, const float *d_scale, const void *d_base,
                     void *d_Y, int dtype, const int *d_adapter_ptr, const int *d_row, int T, int E, int R, int K, int N,

@@ -151,8 +151,9 @@ __device__ __forceinline__ RowTile find_row_tile(const int *__restrict__ ptr, in
     const int a = clamp_place(ptr[lo], M), b = clamp_place(ptr[lo + 1], M);
     RowTile t;
     t.expert = lo;
-    t.first = a + (number - (a / BM + lo)) * BM;
-    t.rows = number < a / BM + lo ? 0 : min(max(b - t.first, 0), BM);
+    const long long first = a + ((long long)number - a / BM - lo) * BM;
+    t.rows = first < a || first >= b ? 0 : min(b - (int)first, BM);
+    t.first = t.rows ? (int)first : a;
     return t;
 }
 // Workgroups are dealt to the 8 dies in turn, each with an L2 of its own.  Runs

@@ -6,7 +6,9 @@ A routing matrix is a sparse matrix of T tokens by E experts with k nonzeros in 
 spmm.py, torch gives device memory and the stream only, every computation is a call through the C ABI, and tensors
 must be contiguous.  Data may be float32, float16 or bfloat16; sums are held in fp32.  Every function takes its result
 tensors as `out` arguments where the caller wants to own them.  Calls run on the current stream of the tensors' device,
-which need not be the current device.  No counterpart in the reference.
+which need not be the current device.  They build no autograd graph: gradients are functions of their own
+(route_backward, experts_mm_dx, experts_mm_dw, combine_backward), to be called in a caller's autograd.Function or
+training step.  No counterpart in the reference.
 """
 import ctypes
 import functools
@@ -105,12 +107,18 @@ def _options(k, score, groups, top_groups, group_score, renormalise, scale):
                                            bool(renormalise), scale))
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(name, *sizes):
+    """mps_<name>(sizes, &bytes)."""
+    need = ctypes.c_size_t()
+    check(getattr(_cabi.lib(), name)(*sizes, ctypes.byref(need)), name)
+    return need.value
+
+
 def _workspace(T, E, k, device):
     """Device memory for the columns of a long routing matrix; None where none is needed."""
-    need = ctypes.c_size_t()
-    check(_cabi.lib().mps_route_workspace_bytes(T, E, k, ctypes.byref(need)), "mps_route_workspace_bytes")
-    ws = torch.empty(need.value, dtype=torch.uint8, device="cuda:%d" % device) if need.value else None
-    return ws, need.value
+    size = _workspace_bytes("mps_route_workspace_bytes", T, E, k)
+    return torch.empty(size, dtype=torch.uint8, device="cuda:%d" % device) if size else None, size
 
 
 def route(scores, k, *, score="softmax", bias=None, groups=1, top_groups=1, group_score="max", renormalise=False,
@@ -131,7 +139,7 @@ def route(scores, k, *, score="softmax", bias=None, groups=1, top_groups=1, grou
         raise ValueError("k must be positive")
     n = T * k
     _fits(n, E)
-    ws, size = (None, 0) if n <= 2048 else _workspace(T, E, k, device)
+    ws, size = _workspace(T, E, k, device) if n > 2048 else (None, 0)  # short ones are known to need none
     if out is None:
         # one allocation: the four arrays of integers, and the weights' bits
         ints = torch.empty(4 * n + E + 1, dtype=torch.int32, device=scores.device)
@@ -306,11 +314,8 @@ def adapters_mm(X, A, B, scale, adapter_ptr, row, *, base=None, out=None):
         _need(base, "base", t, (T, N), device)
     _fits(T, E, R, K, N)
     out = X.new_empty((T, N)) if out is None else _need(out, "out", t, (T, N), device)
-    need = ctypes.c_size_t()
-    status = _cabi.lib().mps_adapters_workspace_bytes(T, E, R, K, ctypes.byref(need))
-    if status:
-        check(status, "mps_adapters_workspace_bytes")
-    ws = torch.empty(max(need.value, 16), dtype=torch.uint8, device=X.device)
+    size = _workspace_bytes("mps_adapters_workspace_bytes", T, E, R, K)
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device=X.device)
     _call("mps_adapters_mm", device, X.data_ptr(), A.data_ptr(), B.data_ptr(), _ptr(scale), _ptr(base), out.data_ptr(),
-          _DTYPES[t], adapter_ptr.data_ptr(), row.data_ptr(), T, E, R, K, N, ws.data_ptr(), need.value)
+          _DTYPES[t], adapter_ptr.data_ptr(), row.data_ptr(), T, E, R, K, N, ws.data_ptr(), size)
     return out

@@ -172,6 +172,77 @@ def test_route_next_to_a_border(r, dev):
     check_routing(m, expert, weight, E)
 
 
+def test_route_groups_next_to_a_border(r, dev):
+    """Groups whose scores differ by 2^-44 or not at all: told apart, and ties to the lower group."""
+    T, E, groups = 20, 64, 8
+    l = torch.zeros(T, E)
+    rank = torch.tensor([3, 1, 3, 0, 2, 1, 0, 3])
+    b = (rank.repeat_interleave(E // groups) * 2.0 ** -45).float()
+    options = dict(score="sigmoid", groups=groups, top_groups=4, group_score="top2")
+    for few in (T, 3):
+        m = r.route(l[:few].to(dev), 28, bias=b.to(dev), **options)
+        expert, weight = exact_route(l[:few].double().numpy(), b.double().numpy(), 28, **options)
+        assert sorted(set(expert[0] // 8)) == [0, 2, 4, 7]
+        check_routing(m, expert, weight, E)
+
+
+@pytest.mark.parametrize("T", [1, 2, 4, 5, 15, 16, 17, 33])
+@pytest.mark.parametrize("E,k,options", [(8, 2, {}), (64, 6, dict(renormalise=True)), (200, 20, dict(score="sigmoid")), (256, 31, {}),
+                                         (256, 8, GROUPED), (300, 32, dict(renormalise=True)), (512, 16, GROUPED), (1024, 9, {})])
+def test_route_few_tokens(r, dev, T, E, k, options):
+    """Around the number of tokens that one launch takes, for every number of experts in a lane."""
+    l = normal(T + k, T, E, t=torch.bfloat16, scale=2.0)
+    l[T // 2] = -np.inf
+    m = r.route(l.to(dev), k, bias=torch.zeros(E, device=dev) if E == 256 else None, **options)
+    expert, weight = exact_route(l.double().numpy(), np.zeros(E) if E == 256 else None, k, **options)
+    check_routing(m, expert, weight, E)
+
+
+def test_no_tokens(r, dev):
+    m = r.route(torch.zeros(0, 16, device=dev), 4)
+    assert m.expert.shape == (0, 4) and m.expert_ptr.cpu().tolist() == [0] * 17
+    W = torch.ones(16, 8, 24, device=dev)
+    assert r.experts_mm(torch.zeros(0, 24, device=dev), W, m.expert_ptr, slot=m.slot, k=4).shape == (0, 8)
+    assert r.experts_mm_dx(torch.zeros(0, 8, device=dev), W, m.expert_ptr).shape == (0, 24)
+    out = torch.full((16, 8, 24), 7.0, device=dev)
+    r.experts_mm_dw(torch.zeros(0, 8, device=dev), torch.zeros(0, 24, device=dev), m.expert_ptr, slot=m.slot, k=4, out=out)
+    assert (out == 0).all()
+    assert r.combine(torch.zeros(0, 24, device=dev), m.pos, m.weight).shape == (0, 24)
+    back = r.combine_backward(torch.zeros(0, 24, device=dev), torch.zeros(0, 24, device=dev), m.weight, m.expert_ptr, m.slot)
+    assert back["dZ"].shape == (0, 24) and back["dweight"].shape == (0, 4)
+    assert r.route_backward(torch.zeros(0, 16, device=dev), m.expert, m.weight).shape == (0, 16)
+    A, B = torch.zeros(3, 8, 24, device=dev), torch.zeros(3, 8, 8, device=dev)
+    ptr, row, _ = r.columns(torch.zeros(0, 1, dtype=torch.int32, device=dev), 3)
+    assert r.adapters_mm(torch.zeros(0, 24, device=dev), A, B, None, ptr, row).shape == (0, 8)
+
+
+def test_results_in_the_callers_tensors(r, dev):
+    l = normal(1, 30, 24).to(dev)
+    ref = r.route(l, 3)
+    out = r.Routing(*(torch.full_like(x, 77) for x in ref))
+    assert r.route(l, 3, out=out) is out
+    for a, b in zip(out, ref):
+        assert torch.equal(a, b)
+    with pytest.raises(ValueError):
+        r.route(l, 4, out=out)
+
+
+def test_tables_that_do_not_fit_reach_nothing_outside(r, dev):
+    """expert_ptr beyond the places, falling, or negative: clamped.  The results mean nothing, but what lies behind them
+    is not touched."""
+    M, N, K = 40, 24, 32
+    X, W, dY = normal(1, M, K).to(dev), normal(2, 3, N, K).to(dev), normal(3, M, N).to(dev)
+    for ptr in ([0, 10, 1000, 2000], [-5, 20, 10, 40], [30, 20, 10, 0], [0, 0, 0, 2 ** 31 - 1], [50, 60, 70, 80]):
+        p = torch.tensor(ptr, dtype=torch.int32, device=dev)
+        buf = torch.full((M + 8, N), 7.0, device=dev)
+        r.experts_mm(X, W, p, out=buf[:M])
+        assert (buf[M:] == 7.0).all()
+        buf = torch.full((M + 8, K), 7.0, device=dev)
+        r.experts_mm_dx(dY, W, p, out=buf[:M])
+        assert (buf[M:] == 7.0).all()
+        assert r.experts_mm_dw(dY, X, p).shape == (3, N, K)
+
+
 def test_route_nan_shows(r, dev):
     l = normal(3, 6, 40)
     l[1, 7] = np.nan
