@@ -34,12 +34,6 @@ class Routing(NamedTuple):
     pos: torch.Tensor
 
 
-def _is(t, dtype, shape, device):
-    """Whether t is a contiguous tensor of this type and shape on GPU number `device`."""
-    return (isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.get_device() == device
-            and device >= 0 and t.is_contiguous())
-
-
 def _first(t, name, dims):
     """The operand that says of which type and on which device the others are: (type, device)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -54,7 +48,8 @@ def _first(t, name, dims):
 
 
 def _need(t, name, dtype, shape, device):
-    if _is(t, dtype, shape, device):
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device
+            and device >= 0 and t.is_contiguous()):
         return t
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("%s must be a CUDA/HIP torch tensor" % name)
@@ -76,22 +71,27 @@ def _shape_of(t, name, dims):
 
 def _fits(*sizes):
     """Sizes travel as 32-bit ints; a larger one must not come out as another number."""
-    if max(sizes) > 0x7FFFFFFF or min(sizes) < 0:
-        check(_cabi.MPS_ERR_UNSUPPORTED, "sizes beyond 32 bits")
+    for n in sizes:
+        if not 0 <= n <= 0x7FFFFFFF:
+            check(_cabi.MPS_ERR_UNSUPPORTED, "sizes beyond 32 bits")
 
 
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+@functools.lru_cache(maxsize=None)
+def _entry(name):
+    return getattr(_cabi.lib(), name)
+
+
 def _call(name, device, *args):
     """mps_<name>(args, stream) on GPU number `device`, on the stream that is current there."""
-    fn = getattr(_cabi.lib(), name)
-    if device == torch.cuda.current_device():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if device == torch._C._cuda_getDevice():
+        status = _entry(name)(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+            status = _entry(name)(*args, torch._C._cuda_getCurrentRawStream(device))
     if status:
         check(status, name)
 
@@ -141,12 +141,12 @@ def route(scores, k, *, score="softmax", bias=None, groups=1, top_groups=1, grou
     _fits(n, E)
     ws, size = _workspace(T, E, k, device) if n > 2048 else (None, 0)  # short ones are known to need none
     if out is None:
-        # one allocation: the four arrays of integers, and the weights' bits
-        ints = torch.empty(4 * n + E + 1, dtype=torch.int32, device=scores.device)
-        expert, weight, pos, slot, expert_ptr = ints.split_with_sizes((n, n, n, n, E + 1))
-        out = Routing(expert.view(T, k), weight.view(torch.float32).view(T, k), expert_ptr, slot, pos.view(T, k))
+        # one allocation for all that is as long as there are slots, the weights' bits among them
+        ints = scores.new_empty((4, T, k), dtype=torch.int32)
+        expert, weight, slot, pos = ints.unbind()
+        out = Routing(expert, weight.view(torch.float32), scores.new_empty((E + 1,), dtype=torch.int32), slot.view(n), pos)
         at = ints.data_ptr()
-        at = at, at + 4 * n, at + 16 * n, at + 12 * n, at + 8 * n
+        at = at, at + 4 * n, out.expert_ptr.data_ptr(), at + 8 * n, at + 12 * n
     else:
         _need(out.expert, "expert", torch.int32, (T, k), device)
         _need(out.weight, "weight", torch.float32, (T, k), device)
