@@ -87,10 +87,27 @@ __device__ __forceinline__ void wave_sync()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// As written, without the steps that the compiler adds for NaN.
+__device__ __forceinline__ double max_f64(double a, double b)
+{
+    double r;
+    asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ double min_f64(double a, double b)
+{
+    double r;
+    asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
 // exp(x) for x <= 0 to about 2^-46 of itself: 2^n times the first twelve terms of
-// the series at |r| <= log(2) / 2, whose remainder is r^12 / 12! < 7e-15.
+// the series at |r| <= log(2) / 2, whose remainder is r^12 / 12! < 7e-15.  No
+// branches, so that a lane's exponentials go side by side and share their
+// constants.  Below -700, and for NaN, exp(-700): the caller sees to NaN.
 __device__ __forceinline__ double exp_wide(double x)
 {
+    x = max_f64(x, -700.0);
     const double n = __builtin_rint(x * 1.4426950408889634074);
     double r = __builtin_fma(n, -6.93147180369123816490e-01, x);  // the first 32 bits of log(2), and the rest
     r = __builtin_fma(n, -1.90821492927058770002e-10, r);
@@ -106,7 +123,7 @@ __device__ __forceinline__ double exp_wide(double x)
     p = __builtin_fma(p, r, 0.5);
     p = __builtin_fma(p, r, 1.0);
     p = __builtin_fma(p, r, 1.0);
-    return x > -700.0 ? __builtin_ldexp(p, (int)n) : x != x ? x : 0.0;
+    return __builtin_ldexp(p, (int)n);
 }
 // 1 / x, 1 <= x <= 2^11: the instruction's estimate, and two of Newton's steps.
 __device__ __forceinline__ double reciprocal_wide(double x)
@@ -144,25 +161,9 @@ __device__ __forceinline__ int expert_of(double v)
 {
     return (int)((high_word(v) >> 31 ? low_word(v) : ~low_word(v)) & 1023u);
 }
-// As written, without the steps that the compiler adds for NaN: there are none.
-__device__ __forceinline__ double max_f64(double a, double b)
-{
-    double r;
-    asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
-__device__ __forceinline__ double min_f64(double a, double b)
-{
-    double r;
-    asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
-// How near two packed choice scores may be and still not be told apart: a score
-// is off by 2^-44 of one at most, the tag by 2^-42 of the whole.
-__device__ __forceinline__ double doubt(double a, double b)
-{
-    return 0x1p-38 * __builtin_fmax(1.0, __builtin_fmax(__builtin_fabs(a), __builtin_fabs(b)));
-}
+// How near a packed choice score may be to this one and still not be told apart:
+// a score is off by 2^-44 of one at most, the tag by 2^-42 of the whole.
+__device__ __forceinline__ double doubt(double a) { return 0x1p-38 * max_f64(1.0, __builtin_fabs(a)); }
 
 // The k best of a token's packed choice scores, held by L lanes with IPL experts
 // each (expert lane * IPL + i).  The j-th choice ends up in lane j.  With
@@ -185,7 +186,7 @@ __device__ __forceinline__ unsigned long long choose(double (&v)[IPL], int k, in
         const double best = fold_group<L>(m[0], max_f64);
         const bool is = high_word(best) != kNeverChosen;
         if constexpr (WATCH) {
-            if (j > 0 && is && last - best <= doubt(last, best)) close |= 1ull << j;
+            if (j > 0 && is && last - best <= doubt(best)) close |= 1ull << j;
             last = best;
         }
         const int e = expert_of(best);
@@ -224,12 +225,12 @@ __device__ __forceinline__ bool keep_group_lanes(double (&v)[IPL], const RouteSh
     const int group = lane / sh.group_lanes;
     if (group < sh.groups && lane % sh.group_lanes == 0) of_group[group] = own;
     wave_sync();
-    int better = 0, near = 0;
+    const double apart = 2.0 * doubt(own);
+    int better = 0, near = WATCH ? -1 : 0;  // the group itself is near
     for (int h = 0; h < sh.groups; ++h) {
         const double x = of_group[h];
         better += x > own || (x == own && h < group);
-        // two groups without experts are equally bad (their difference is NaN)
-        if constexpr (WATCH) near += h != group && __builtin_fabs(x - own) <= 2.0 * doubt(x, own);
+        if constexpr (WATCH) near += __builtin_fabs(x - own) <= apart;
     }
     wave_sync();
     if (better >= sh.top_groups || group >= sh.groups) {
@@ -237,7 +238,7 @@ __device__ __forceinline__ bool keep_group_lanes(double (&v)[IPL], const RouteSh
         for (int i = 0; i < IPL; ++i) v[i] = from_words(kNeverChosen, low_word(v[i]));
     }
     // a kept group that might be behind the border; a group behind it that might be kept is near one
-    return WATCH && group < sh.groups && better < sh.top_groups && better + near >= sh.top_groups;
+    return WATCH && group < sh.groups && better < sh.top_groups && near > 0 && better + near >= sh.top_groups;
 }
 
 // The same choice without shortcuts, with scores in 64 bits and ties by index:
@@ -351,6 +352,7 @@ __device__ __forceinline__ void route_token(const T *__restrict__ row, bool live
         for (int i = 0; i < IPL; ++i) m = max(m, key_of(l[i]));
         largest = of_key(group_max<L>(m));
     }
+    const bool broken = soft && !(largest < __builtin_inff());  // no softmax over NaN or an infinite score
     double v[IPL];
     if (plain) {
 #pragma unroll
@@ -367,9 +369,9 @@ __device__ __forceinline__ void route_token(const T *__restrict__ row, bool live
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < IPL; ++i) {
-            const double x = soft ? (double)l[i] - (double)largest : -__builtin_fabs((double)l[i]);
-            v[i] = l[i] == minus_inf ? 0.0 : exp_wide(x);
-            if (soft) sum += v[i];
+            // -inf counts as exp(-700) in the sum, far below its last bit; it is never chosen
+            v[i] = exp_wide(soft ? (double)l[i] - (double)largest : -__builtin_fabs((double)l[i]));
+            sum += v[i];
         }
         double scale = 1.0;
         if (soft) {
@@ -380,9 +382,8 @@ __device__ __forceinline__ void route_token(const T *__restrict__ row, bool live
 #pragma unroll
         for (int i = 0; i < IPL; ++i) {
             const double r = soft ? scale : reciprocal_wide(1.0 + v[i]);
-            v[i] = soft || l[i] < 0.0f ? v[i] * r : r;
-            v[i] += (double)b[i];
-            if (l[i] == minus_inf) v[i] = -__builtin_inf();
+            const double s = soft || l[i] < 0.0f ? v[i] * r : r;
+            v[i] = l[i] == minus_inf ? -__builtin_inf() : broken || l[i] != l[i] ? __builtin_nan("") : s + (double)b[i];
         }
     }
 #pragma unroll
@@ -417,7 +418,7 @@ __device__ __forceinline__ void route_token(const T *__restrict__ row, bool live
     } else {
         w = lj == minus_inf ? 0.0f : (soft ? exp_near(lj - largest) / total : sigmoid_near(lj));
     }
-    if (soft && !(largest < __builtin_inff())) w = __builtin_nanf("");  // no softmax over NaN or an infinite score
+    if (broken) w = __builtin_nanf("");
     w = e < 0 ? 0.0f : w * sh.scale;
 }
 
