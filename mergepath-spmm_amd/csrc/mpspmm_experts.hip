@@ -271,7 +271,12 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
 
 // The same products where rows are whole 16 bytes.  The stages come straight
 // from memory into LDS, two of them in turn: while the matrix instructions work
-// on one, the other is on its way.
+// on one, the other is on its way.  Measured, 256 x 256 tiles, fp16: 1202 TFLOP/s
+// for one expert of 8192 x 8192 x 8192 (a library product: 1414), 897 for 64
+// experts of 768 rows, 1408 x 2048 (a last tile of half the columns), 840 where
+// their rows are uneven.  Four stages of one matrix step, for requests three
+// ahead, and sums that begin at another place in every column tile gave nothing:
+// neither the way from memory nor its channels bound it.
 //   PP, QP  panels of S in the tile's columns and rows
 //   WP, WQ  wavefronts that share them
 typedef __attribute__((address_space(3))) void *lds_ptr;
