@@ -241,9 +241,56 @@ __device__ __forceinline__ bool keep_group_lanes(double (&v)[IPL], const RouteSh
     return WATCH && group < sh.groups && better < sh.top_groups && near > 0 && better + near >= sh.top_groups;
 }
 
-// The same choice without shortcuts, with scores in 64 bits and ties by index:
-// for tokens that the above leaves in doubt, and for groups that do not fit the
-// lanes.  `all`: sh.E scores of LDS, `of_group`: sh.groups.
+// The same where groups and lanes do not fit each other: a group's scores are
+// read back from LDS by one lane.  `all`: sh.E values of LDS, `of_group`: sh.groups.
+template <int IPL, int L, bool WATCH>
+__device__ __forceinline__ bool keep_groups_apart(double (&v)[IPL], const RouteShape &sh, int lane,
+                                                  double *__restrict__ all, double *__restrict__ of_group)
+{
+#pragma unroll
+    for (int i = 0; i < IPL; ++i)
+        if (lane * IPL + i < sh.E) all[lane * IPL + i] = v[i];
+    wave_sync();
+    for (int g = lane; g < sh.groups; g += L) {
+        double first = from_words(kNeverChosen, 0), second = first;
+        for (int i = 0; i < sh.group_size; ++i) {
+            const double x = all[g * sh.group_size + i];
+            second = max_f64(second, min_f64(first, x));
+            first = max_f64(first, x);
+        }
+        of_group[g] = sh.group_score == MPS_GROUP_TOP2 ? first + second : first;
+    }
+    wave_sync();
+    bool close = false;
+    for (int g = lane; g < sh.groups; g += L) {
+        const double own = of_group[g], apart = 2.0 * doubt(own);
+        int better = 0, near = WATCH ? -1 : 0;  // the group itself is near
+        for (int h = 0; h < sh.groups; ++h) {
+            const double x = of_group[h];
+            better += x > own || (x == own && h < g);
+            if constexpr (WATCH) near += __builtin_fabs(x - own) <= apart;
+        }
+        all[g] = better < sh.top_groups ? 1.0 : 0.0;  // groups <= E; the scores have been read
+        close |= WATCH && better < sh.top_groups && near > 0 && better + near >= sh.top_groups;
+    }
+    wave_sync();
+    int g = lane * IPL / sh.group_size, left = (g + 1) * sh.group_size - lane * IPL;
+#pragma unroll
+    for (int i = 0; i < IPL; ++i) {
+        if (left == 0) {
+            ++g;
+            left = sh.group_size;
+        }
+        --left;
+        if (g >= sh.groups || all[min(g, sh.groups - 1)] == 0.0) v[i] = from_words(kNeverChosen, low_word(v[i]));
+    }
+    wave_sync();
+    return close;
+}
+
+// The same choice without shortcuts, with scores in 64 bits and ties by index,
+// for tokens that the above leaves in doubt.  `all`: sh.E scores of LDS,
+// `of_group`: sh.groups.
 template <typename T, int IPL, int L>
 __device__ __forceinline__ int choose_again(const T *__restrict__ row, bool live, const float *__restrict__ bias,
                                             const RouteShape &sh, int lane, bool plain, float largest,
@@ -388,14 +435,16 @@ __device__ __forceinline__ void route_token(const T *__restrict__ row, bool live
     }
 #pragma unroll
     for (int i = 0; i < IPL; ++i) v[i] = pack_choice(v[i], lane * IPL + i);
-    bool again = sh.groups > 1 && sh.group_lanes == 0;
-    if (!again) {
-        double *of_group = reinterpret_cast<double *>(mine + sh.E);
+    bool again = false;
+    {
+        double *all = reinterpret_cast<double *>(mine), *of_group = all + sh.E;
         if (plain) {
-            if (sh.groups > 1) keep_group_lanes<IPL, L, false>(v, sh, lane, of_group);
+            if (sh.groups > 1 && sh.group_lanes) keep_group_lanes<IPL, L, false>(v, sh, lane, of_group);
+            else if (sh.groups > 1) keep_groups_apart<IPL, L, false>(v, sh, lane, all, of_group);
             choose<IPL, L, false>(v, sh.k, lane, e);
         } else {
-            if (sh.groups > 1) again = keep_group_lanes<IPL, L, true>(v, sh, lane, of_group);
+            if (sh.groups > 1 && sh.group_lanes) again = keep_group_lanes<IPL, L, true>(v, sh, lane, of_group);
+            else if (sh.groups > 1) again = keep_groups_apart<IPL, L, true>(v, sh, lane, all, of_group);
             const unsigned long long close = choose<IPL, L, true>(v, sh.k, lane, e);
             if (__any(close != 0)) {
                 const float le = e >= 0 ? (float)row[e] : 0.0f, be = e >= 0 && bias ? bias[e] : 0.0f;
@@ -850,7 +899,7 @@ RouteShape make_shape(const mps_route_options &o, int T, int E)
 
 // Lanes and experts per lane for a token: 16 lanes do four tokens in a wavefront,
 // and their maxima cross lanes in four cheap steps (16384 tokens of 256 experts
-// with a bias and groups: 23 us on the GPU, 43 with 64 lanes and scores in 32
+// with a bias and groups: 21 us on the GPU, 43 with 64 lanes and scores in 32
 // bits); more where the experts or the choices need them.
 template <typename F>
 int with_route_lanes(const RouteShape &sh, F &&f)
