@@ -91,8 +91,8 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_shrink_kernel(const T *_
 // made in fp32; for the product with B it is split into its rounding to T and
 // the rounding of what that leaves, two instructions instead of one, so that
 // it is not rounded to 8 or 11 bits on the way.  fp16 has no room for values
-// from 65520 on: where a tile holds one, all of its V are taken down by 2^16
-// and the sums up again.  RANK: the largest rank, in units of 32.
+// from 65520 on: where a token has one, all of its V are taken down by 2^16
+// and its sums up again.  RANK: the largest rank, in units of 32.
 // Row g * 4 + d of the b-th matrix instruction is the column that leaves a lane
 // with 16 bytes of neighbouring columns, and the four lanes of a token with 64.
 template <typename T, int RANK, int MT, bool ALIGNED>
@@ -156,8 +156,8 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
                     far |= __builtin_fabsf(v[step][c]) > 65000.0f;
                 }
             }
-            // 16 tokens share a scale; the other 16s of a tile have their own
-            const bool take = __is_same(T, half_t) && __any(far);
+            // a token's values lie in the four lanes i, i + 16, i + 32, i + 48; its sums come back to the same lanes
+            const bool take = __is_same(T, half_t) && (__ballot(far) >> i & 0x0001000100010001ull) != 0;
 #pragma unroll
             for (int step = 0; step < STEPS; ++step) {
                 T high_of[C], low_of[C];

@@ -636,6 +636,15 @@ def test_adapters_beyond_the_range_of_fp16(r, dev):
     ptr, row, _ = r.columns(torch.zeros(T, 1, dtype=torch.int32, device=dev), 1)
     out = r.adapters_mm(X.to(dev), A.to(dev), B.to(dev), None, ptr, row)
     assert (out.cpu() == 64 * 8 * 256 * 8 / 1024).all()
+    # one token's large values take no bits from its neighbours'
+    X = normal(1, T, K, t=torch.float16, scale=0.01)
+    B2 = normal(2, 1, N, 8, t=torch.float16)
+    alone = r.adapters_mm(X.to(dev), A.to(dev), B2.to(dev), None, ptr, row).cpu()
+    X[3] = 64.0
+    beside = r.adapters_mm(X.to(dev), A.to(dev), B2.to(dev), None, ptr, row).cpu()
+    others = torch.arange(T) != 3
+    assert torch.equal(alone[others], beside[others])
+    X = torch.full((T, K), 64.0, dtype=torch.float16)
     X[3, 9] = np.inf
     out = r.adapters_mm(X.to(dev), A.to(dev), B.to(dev), None, ptr, row).cpu()
     assert torch.isinf(out[3]).all() and (out[[0, 1, 2, 4, 19]] == 1024.0).all()
