@@ -825,10 +825,11 @@ __global__ __launch_bounds__(256) void combine_kernel(const T *__restrict__ Z, c
     store_vec<T, V, ALIGNED>(Y + t * N + col, acc, valid);
 }
 
-// One wavefront per place: reads the row of Z and the token's row of dY, writes
-// the row of dZ and the product of the two rows.  Places are in order, so Z and
-// dZ stream; the k reads of a row of dY meet in the caches.
-template <typename T, bool ALIGNED>
+// L lanes per place, a wavefront or for narrow rows less: they read the row of Z
+// and the token's row of dY, write the row of dZ and the product of the two
+// rows.  Places are in order, so Z and dZ stream; the k reads of a row of dY meet
+// in the caches.
+template <typename T, int L, bool ALIGNED>
 __global__ __launch_bounds__(256) void combine_backward_kernel(const T *__restrict__ dY, const T *__restrict__ Z,
                                                                const float *__restrict__ weight,
                                                                const int *__restrict__ expert_ptr, int E,
@@ -836,9 +837,10 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T *__restri
                                                                float *__restrict__ dweight, int k, int M, int N)
 {
     constexpr int V = 16 / sizeof(T);
-    const int lane = threadIdx.x & 63;
-    const int p = (int)min((long long)blockIdx.x * 4 + (threadIdx.x >> 6), (long long)M);
-    if (p >= M) return;
+    const int lane = threadIdx.x & (L - 1);
+    const long long at = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (at >= M) return;
+    const int p = (int)at;
     const int s = slot[p];
     const bool known = (unsigned)s < (unsigned)M;
     const bool routed = known && p < expert_ptr[E];
@@ -848,19 +850,19 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T *__restri
     T *out = dZ + (long long)p * N;
     // A load behind a store waits for it, so that several chunks of both rows are
     // loaded before any is stored.
-    constexpr int U = 4;
+    constexpr int U = L == 64 ? 4 : 1;
     float dot = 0.0f;
-    for (int first = lane * V; first < N; first += U * 64 * V) {
+    for (int first = lane * V; first < N; first += U * L * V) {
         float y[U][V], z[U][V];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int col = first + u * 64 * V;
+            const int col = first + u * L * V;
             load_vec<T, V, ALIGNED>(y[u], y_row + col, routed ? N - col : 0);
             load_vec<T, V, ALIGNED>(z[u], z_row + col, routed && dweight ? N - col : 0);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int col = first + u * 64 * V;
+            const int col = first + u * L * V;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 dot = __builtin_fmaf(y[u][i], z[u][i], dot);
@@ -870,7 +872,7 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T *__restri
         }
     }
     if (dweight && known) {
-        dot = group_sum<64>(dot);
+        dot = group_sum<L>(dot);
         if (lane == 0) dweight[s] = routed ? dot : 0.0f;
     }
 }
@@ -977,12 +979,19 @@ int launch_combine_backward(const void *dY, const void *Z, const float *weight, 
                             const int *slot, void *dZ, float *dweight, int k, int M, int N, hipStream_t st)
 {
     const bool fast = rows_of_16(dY, N, sizeof(T)) && rows_of_16(Z, N, sizeof(T)) && rows_of_16(dZ, N, sizeof(T));
-#define MPS_LAUNCH_COMBINE(ALIGNED)                                                                                \
-    hipLaunchKernelGGL((combine_backward_kernel<T, ALIGNED>), dim3(ceil_div(M, 4)), dim3(256), 0, st,              \
+    const int chunks = ceil_div(N, 16 / (int)sizeof(T));
+#define MPS_LAUNCH_COMBINE(L, ALIGNED)                                                                             \
+    hipLaunchKernelGGL((combine_backward_kernel<T, L, ALIGNED>), dim3(ceil_div(M, 256 / L)), dim3(256), 0, st,     \
                        static_cast<const T *>(dY), static_cast<const T *>(Z), weight, expert_ptr, E, slot,         \
                        static_cast<T *>(dZ), dweight, k, M, N)
-    if (fast) MPS_LAUNCH_COMBINE(true);
-    else MPS_LAUNCH_COMBINE(false);
+#define MPS_LAUNCH_LANES(L)                     \
+    if (fast) MPS_LAUNCH_COMBINE(L, true);      \
+    else MPS_LAUNCH_COMBINE(L, false)
+    if (chunks <= 8) { MPS_LAUNCH_LANES(8); }
+    else if (chunks <= 16) { MPS_LAUNCH_LANES(16); }
+    else if (chunks <= 32) { MPS_LAUNCH_LANES(32); }
+    else { MPS_LAUNCH_LANES(64); }
+#undef MPS_LAUNCH_LANES
 #undef MPS_LAUNCH_COMBINE
     MPS_HIP_TRY(hipGetLastError());
     return MPS_OK;

@@ -543,7 +543,8 @@ def routing_of(T, E, k, none, seed):
 
 @pytest.mark.parametrize("t", list(TYPES))
 @pytest.mark.parametrize("T,E,k,N,none", [(1, 2, 1, 1, 0.0), (3, 4, 4, 8, 0.3), (70, 16, 6, 1030, 0.1), (129, 9, 5, 264, 0.0),
-                                          (17, 8, 8, 4097, 0.5), (5, 3, 2, 16, 1.0)])
+                                          (17, 8, 8, 4097, 0.5), (5, 3, 2, 16, 1.0), (67, 5, 3, 39, 0.2), (40, 6, 4, 64, 0.1),
+                                          (33, 4, 2, 121, 0.1), (21, 7, 5, 250, 0.3), (9, 2, 1, 512, 0.0)])
 def test_combine(r, dev, t, T, E, k, N, none):
     t = TYPES[t]
     ptr, slot, pos = routing_of(T, E, k, none, T + N)
