@@ -979,6 +979,7 @@ int launch_combine_backward(const void *dY, const void *Z, const float *weight, 
                             const int *slot, void *dZ, float *dweight, int k, int M, int N, hipStream_t st)
 {
     const bool fast = rows_of_16(dY, N, sizeof(T)) && rows_of_16(Z, N, sizeof(T)) && rows_of_16(dZ, N, sizeof(T));
+    // as many lanes as a row has chunks (34076 places of 39 columns bf16: 10.6 us a call, 29.7 with 64)
     const int chunks = ceil_div(N, 16 / (int)sizeof(T));
 #define MPS_LAUNCH_COMBINE(L, ALIGNED)                                                                             \
     hipLaunchKernelGGL((combine_backward_kernel<T, L, ALIGNED>), dim3(ceil_div(M, 256 / L)), dim3(256), 0, st,     \
