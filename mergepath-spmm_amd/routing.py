@@ -12,6 +12,7 @@ training step.  No counterpart in the reference.
 """
 import ctypes
 import functools
+import operator
 from typing import NamedTuple
 
 import torch
@@ -96,15 +97,21 @@ def _call(name, device, *args):
         check(status, name)
 
 
-@functools.lru_cache(maxsize=64)
 def _options(k, score, groups, top_groups, group_score, renormalise, scale):
-    """mps_route_options, as an argument of a call.  The structure is only read."""
+    """mps_route_options, as an argument of a call.  Kept by the numbers that it holds: what the caller gives may be a
+    tensor, whose value changes in place."""
     if score not in _SCORES:
         raise ValueError("score must be one of %s" % sorted(_SCORES))
     if group_score not in _GROUP_SCORES:
         raise ValueError("group_score must be one of %s" % sorted(_GROUP_SCORES))
-    return ctypes.byref(_cabi.RouteOptions(k, _SCORES[score], groups, top_groups, _GROUP_SCORES[group_score],
-                                           bool(renormalise), scale))
+    return _options_of(operator.index(k), _SCORES[score], operator.index(groups), operator.index(top_groups),
+                       _GROUP_SCORES[group_score], bool(renormalise), ctypes.c_float(scale).value)
+
+
+@functools.lru_cache(maxsize=64)
+def _options_of(*numbers):
+    """The structure is only read."""
+    return ctypes.byref(_cabi.RouteOptions(*numbers))
 
 
 @functools.lru_cache(maxsize=256)
@@ -132,6 +139,7 @@ def route(scores, k, *, score="softmax", bias=None, groups=1, top_groups=1, grou
     slot that finds no expert holds -1, weight 0 and pos -1."""
     t, device = _first(scores, "scores", 2)
     T, E = scores.shape
+    k = operator.index(k)
     opt = _options(k, score, groups, top_groups, group_score, renormalise, scale)
     if bias is not None:
         _need(bias, "bias", torch.float32, (E,), device)

@@ -125,3 +125,29 @@ def test_tensors_on_the_host_are_refused(pkg):
         r.columns(torch.zeros(2, 1, dtype=torch.int32), 3)
     with pytest.raises(TypeError):
         r.combine(torch.zeros(2, 4), torch.zeros(2, 1, dtype=torch.int32))
+
+
+def test_route_options_are_values(pkg):
+    """A scale that is a tensor counts with the value that it has at the call, also after it was changed in place."""
+    def of(**o):
+        a = dict(k=8, score="softmax", groups=1, top_groups=1, group_score="max", renormalise=False, scale=1.0)
+        a.update(o)
+        return pkg.routing._options(**a)._obj
+
+    scale = torch.nn.Parameter(torch.tensor(2.5))
+    assert of(scale=scale).scale == 2.5
+    with torch.no_grad():
+        scale.fill_(4.0)
+    assert of(scale=scale).scale == 4.0
+    flag = torch.tensor(False)
+    assert of(renormalise=flag).renormalise == 0
+    flag.fill_(True)
+    assert of(renormalise=flag).renormalise == 1
+    k = torch.tensor(3)
+    assert of(k=k).k == 3
+    k.fill_(4)
+    assert of(k=k).k == 4
+    assert of(k=1, groups=1, scale=1).k == 1 and of(k=True, groups=1, scale=1.0).scale == 1.0
+    for bad in (dict(k=2.5), dict(groups="2"), dict(scale="x"), dict(scale=None)):
+        with pytest.raises((TypeError, ValueError)):
+            of(**bad)
