@@ -671,7 +671,7 @@ typedef struct mps_route_options {
  *   s = softmax(l) over all E experts, or sigmoid(l);
  *   c = s + d_bias (d_bias: float[E] or NULL), in the precision of 64 bits;
  *   the top_groups groups with the largest group score stay (ties: the lower
- *   group), and among their experts the k with the largest c are chosen
+ *   group; a sum of two is -inf where the group has no two experts), and among their experts the k with the largest c are chosen
  *   (ties: the lower expert), in descending order of c;
  *   weight = scale * s, or scale * s / (sum of the chosen s).
  * Without a bias c orders as l does, and l itself is compared.  An expert with

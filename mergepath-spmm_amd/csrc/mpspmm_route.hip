@@ -165,6 +165,23 @@ __device__ __forceinline__ int expert_of(double v)
 // a score is off by 2^-44 of one at most, the tag by 2^-42 of the whole.
 __device__ __forceinline__ double doubt(double a) { return 0x1p-38 * max_f64(1.0, __builtin_fabs(a)); }
 
+// The sum of a group's two largest packed choice scores.  Stand-ins are no
+// numbers to add: the sum is that of the values which they stand for (-inf where
+// the group has one expert or none, inf - inf = NaN), one stand-in for each, so
+// that groups with the same sum tie.
+__device__ __forceinline__ double sum_of_two(double first, double second)
+{
+    const unsigned a = high_word(first), b = high_word(second);
+    const unsigned stands = a == kNotANumber || (a == kInfinite && b == kNeverChosen) ? kNotANumber
+                            : b == kNeverChosen                                       ? kNeverChosen
+                            : a == kInfinite                                          ? kInfinite
+                                                                                      : 0;
+    return stands ? from_words(stands, 0) : first + second;
+}
+// How near another group's score may be to this one and still not be told apart.
+// What a stand-in stands for is known: nothing is near it.
+__device__ __forceinline__ double group_doubt(double own) { return __builtin_fabs(own) > 1e300 ? -1.0 : 2.0 * doubt(own); }
+
 // The k best of a token's packed choice scores, held by L lanes with IPL experts
 // each (expert lane * IPL + i).  The j-th choice ends up in lane j.  With
 // WATCH the (k + 1)-th too; returned are the places j whose choice is too near
@@ -221,16 +238,16 @@ __device__ __forceinline__ bool keep_group_lanes(double (&v)[IPL], const RouteSh
     MPS_MERGE_STEP(1) MPS_MERGE_STEP(2) MPS_MERGE_STEP(4) MPS_MERGE_STEP(8) MPS_MERGE_STEP(16) MPS_MERGE_STEP(32)
 #undef MPS_MERGE_STEP
     // the largest members carry their experts' numbers, so that of equal groups the lower is larger
-    const double own = sh.group_score == MPS_GROUP_TOP2 ? first + second : first;
+    const double own = sh.group_score == MPS_GROUP_TOP2 ? sum_of_two(first, second) : first;
     const int group = lane / sh.group_lanes;
     if (group < sh.groups && lane % sh.group_lanes == 0) of_group[group] = own;
     wave_sync();
-    const double apart = 2.0 * doubt(own);
-    int better = 0, near = WATCH ? -1 : 0;  // the group itself is near
+    const double apart = group_doubt(own);
+    int better = 0, near = 0;
     for (int h = 0; h < sh.groups; ++h) {
         const double x = of_group[h];
         better += x > own || (x == own && h < group);
-        if constexpr (WATCH) near += __builtin_fabs(x - own) <= apart;
+        if constexpr (WATCH) near += h != group && __builtin_fabs(x - own) <= apart;
     }
     wave_sync();
     if (better >= sh.top_groups || group >= sh.groups) {
@@ -258,17 +275,17 @@ __device__ __forceinline__ bool keep_groups_apart(double (&v)[IPL], const RouteS
             second = max_f64(second, min_f64(first, x));
             first = max_f64(first, x);
         }
-        of_group[g] = sh.group_score == MPS_GROUP_TOP2 ? first + second : first;
+        of_group[g] = sh.group_score == MPS_GROUP_TOP2 ? sum_of_two(first, second) : first;
     }
     wave_sync();
     bool close = false;
     for (int g = lane; g < sh.groups; g += L) {
-        const double own = of_group[g], apart = 2.0 * doubt(own);
-        int better = 0, near = WATCH ? -1 : 0;  // the group itself is near
+        const double own = of_group[g], apart = group_doubt(own);
+        int better = 0, near = 0;
         for (int h = 0; h < sh.groups; ++h) {
             const double x = of_group[h];
             better += x > own || (x == own && h < g);
-            if constexpr (WATCH) near += __builtin_fabs(x - own) <= apart;
+            if constexpr (WATCH) near += h != g && __builtin_fabs(x - own) <= apart;
         }
         all[g] = better < sh.top_groups ? 1.0 : 0.0;  // groups <= E; the scores have been read
         close |= WATCH && better < sh.top_groups && near > 0 && better + near >= sh.top_groups;

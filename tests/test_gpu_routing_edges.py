@@ -1,0 +1,106 @@
+"""Sparse routing at its edges: masked groups, NaN and infinities in the choice, small and large values between the two
+products of an adapter, sizes beyond one launch's threads, and the kernels' shapes one by one."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_routing import GROUPED, TYPES, check_routing, close, exact_columns, gen, half, normal, routing_of, segments
+from test_gpu_routing import shuffled_slots, weights_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def r(pkg, dev):
+    return pkg.routing
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# The choice among groups that a mask leaves with one expert or with none, NaN, infinities
+# ---------------------------------------------------------------------------------------------------------------------
+
+def rank(c):
+    """Order of choice scores: NaN above everything."""
+    return (1, 0.0) if np.isnan(c) else (0, c)
+
+
+def exact_choice(l, bias, k, score, groups, top_groups, group_score):
+    """Experts of one token, from the definition: c = s + bias, -inf where the score or the bias is; a group counts as the
+    largest of its c or as the sum of the two largest, by the arithmetic of infinities; ties to the lower index."""
+    can = ~((l == -np.inf) | (bias == -np.inf))
+    with np.errstate(all="ignore"):
+        if score == "sigmoid":
+            s = 1.0 / (1.0 + np.exp(-l))
+        elif np.isnan(l).any() or l.max() == np.inf:
+            s = np.full(l.shape, np.nan)
+        else:
+            s = np.where(l > -np.inf, np.exp(l - l.max()), 0.0) if l.max() > -np.inf else np.zeros(l.shape)
+            s = s / s.sum() if s.sum() else s
+        c = np.where(can, s + bias, -np.inf)
+        of = []
+        for g in c.reshape(groups, -1):
+            best = sorted(g, key=rank, reverse=True)
+            of.append(best[0] if group_score == "max" else best[0] + best[1])
+    kept = sorted(range(groups), key=lambda g: rank(of[g]), reverse=True)[:top_groups]
+    at = [e for e in range(len(l)) if e * groups // len(l) in kept and c[e] != -np.inf]
+    at = sorted(at, key=lambda e: rank(c[e]), reverse=True)[:k]
+    return at + [-1] * (k - len(at))
+
+
+LAYOUTS = [(8, 2, 1, 2), (64, 8, 4, 6), (256, 8, 4, 8), (72, 6, 3, 9), (90, 18, 5, 7), (320, 64, 9, 5), (512, 4, 2, 31),
+           (1024, 16, 3, 32)]  # experts, groups, kept ones, k: groups in whole lanes and others
+
+
+def masked_groups(seed, T, E, groups):
+    """Scores of which the mask leaves every group none, one, two or all of its experts."""
+    g = np.random.default_rng(seed)
+    l = g.normal(size=(T, groups, E // groups)).astype(np.float32)
+    for t in range(T):
+        for h in range(groups):
+            left = g.choice([0, 1, 1, 2, E // groups], p=[0.3, 0.2, 0.2, 0.2, 0.1])
+            l[t, h, g.permutation(E // groups)[left:]] = -np.inf
+    return l.reshape(T, E)
+
+
+def check_choice(m, l, bias, k, score, groups, top_groups, group_score="top2"):
+    bias = np.zeros(l.shape[1]) if bias is None else bias.astype(np.float64)
+    ref = np.array([exact_choice(x, bias, k, score, groups, top_groups, group_score) for x in l.astype(np.float64)], np.int32)
+    assert np.array_equal(m.expert.cpu().numpy(), ref)
+    for got, x in zip((m.expert_ptr, m.slot, m.pos), exact_columns(ref, l.shape[1])):
+        assert np.array_equal(got.cpu().numpy(), x)
+    return ref
+
+
+@pytest.mark.parametrize("T", [1, 4, 33])
+@pytest.mark.parametrize("E,groups,top_groups,k", LAYOUTS)
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_groups_that_a_mask_leaves_with_few_experts(r, dev, T, E, groups, top_groups, k, score, biased):
+    """With the sum of the two largest a group with one expert left counts as one with none: -inf, and the lower group
+    comes first.  No token has a tie of finite sums."""
+    l = masked_groups(E + T, T, E, groups)
+    bias = np.random.default_rng(E).normal(size=E).astype(np.float32) * 0.1 if biased else None
+    for group_score in ("top2", "max"):
+        m = r.route(torch.from_numpy(l).to(dev), k, score=score, bias=torch.from_numpy(bias).to(dev) if biased else None,
+                    groups=groups, top_groups=top_groups, group_score=group_score)
+        if group_score == "max" and not biased:  # l itself is compared, which is the same where nothing saturates
+            check_choice(m, l, None, k, "sigmoid", groups, top_groups, "max")
+        else:
+            check_choice(m, l, bias, k, score, groups, top_groups, group_score)
+
+
+@pytest.mark.parametrize("T", [1, 4, 33])
+@pytest.mark.parametrize("E,groups,top_groups,k", LAYOUTS)
+@pytest.mark.parametrize("group_score", ["top2", "max"])
+def test_groups_with_nan_and_infinities(r, dev, T, E, groups, top_groups, k, group_score):
+    """NaN scores (one or two of a group, beside masked ones too) and infinite biases: classes of their own, the larger
+    first, ties to the lower group and expert."""
+    g = np.random.default_rng(E + 7 * T)
+    l = masked_groups(E + 1, T, E, groups)
+    for t in range(T):
+        l[t, g.integers(0, E, size=g.integers(0, 4))] = np.nan
+    bias = g.normal(size=E).astype(np.float32) * 0.1
+    bias[g.integers(0, E, size=3)] = np.inf
+    m = r.route(torch.from_numpy(l).to(dev), k, score="sigmoid", bias=torch.from_numpy(bias).to(dev), groups=groups,
+                top_groups=top_groups, group_score=group_score)
+    check_choice(m, l, bias, k, "sigmoid", groups, top_groups, group_score)
