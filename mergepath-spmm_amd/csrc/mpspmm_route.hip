@@ -471,7 +471,11 @@ __device__ __forceinline__ void route_token(const T *__restrict__ row, bool live
             if (lane >= sh.k) e = -1;
         }
     }
-    if (__any(again && live)) e = choose_again<T, IPL, L>(row, live, bias, sh, lane, plain, largest, mine, mine + sh.E);
+    // All tokens of the wavefront go along; one that is not in doubt keeps what it has.
+    if (__any(again && live)) {
+        const int other = choose_again<T, IPL, L>(row, live, bias, sh, lane, plain, largest, mine, mine + sh.E);
+        if (group_max<L>((unsigned)again)) e = other;
+    }
     // Lane j weighs the j-th choice.
     const float lj = live && lane < sh.k && e >= 0 ? (float)row[e] : minus_inf;
     if (sh.renormalise) {

@@ -104,3 +104,22 @@ def test_groups_with_nan_and_infinities(r, dev, T, E, groups, top_groups, k, gro
     m = r.route(torch.from_numpy(l).to(dev), k, score="sigmoid", bias=torch.from_numpy(bias).to(dev), groups=groups,
                 top_groups=top_groups, group_score=group_score)
     check_choice(m, l, bias, k, "sigmoid", groups, top_groups, group_score)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("E,groups,top_groups,k", LAYOUTS)
+def test_a_token_does_not_depend_on_its_neighbours(r, dev, score, biased, E, groups, top_groups, k):
+    """Rows with masks beside a few with ties, which are chosen with every bit of a double: in another order every row has
+    the same experts and the same weights, bit for bit."""
+    T = 256
+    l = torch.from_numpy(masked_groups(E, T, E, groups))
+    l[::16] = 0.5
+    bias = torch.zeros(E, device=dev) if biased else None
+    options = dict(score=score, bias=bias, groups=groups, top_groups=top_groups, group_score="top2")
+    m = r.route(l.to(dev), k, **options)
+    for seed in range(3):
+        order = torch.randperm(T, generator=gen(seed))
+        other = r.route(l[order].to(dev), k, **options)
+        assert torch.equal(other.expert, m.expert[order.to(dev)])
+        assert torch.equal(other.weight, m.weight[order.to(dev)])
