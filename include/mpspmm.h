@@ -675,8 +675,8 @@ typedef struct mps_route_options {
  *   (ties: the lower expert), in descending order of c;
  *   weight = scale * s, or scale * s / (sum of the chosen s).
  * Without a bias c orders as l does, and l itself is compared.  An expert with
- * l = -inf (or a bias of -inf) is never chosen; slots that find no expert hold
- * -1 and weight 0, also where renormalised.  A NaN counts as the largest
+ * l = -inf or a bias of -inf is never chosen; slots that find no expert hold
+ * -1 and weight 0, also where renormalised.  Else a NaN counts as the largest
  * value, as does what is computed from one, so that it shows in the weights.
  * d_expert_ptr, d_slot, d_pos: all three or all NULL (the rows alone).
  * The workspace is needed for the columns only. */

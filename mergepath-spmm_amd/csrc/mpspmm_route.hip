@@ -333,7 +333,7 @@ __device__ __forceinline__ int choose_again(const T *__restrict__ row, bool live
         double c = (double)l;
         if (!plain && l != minus_inf) {
             c = soft ? exp(c - (double)largest) / sum : 1.0 / (1.0 + exp(-c));
-            if (bias) c += (double)bias[x];
+            if (bias) c = bias[x] == minus_inf ? -__builtin_inf() : c + (double)bias[x];
         }
         key[i] = key_of(c);
     }
@@ -447,7 +447,10 @@ __device__ __forceinline__ void route_token(const T *__restrict__ row, bool live
         for (int i = 0; i < IPL; ++i) {
             const double r = soft ? scale : reciprocal_wide(1.0 + v[i]);
             const double s = soft || l[i] < 0.0f ? v[i] * r : r;
-            v[i] = l[i] == minus_inf ? -__builtin_inf() : broken || l[i] != l[i] ? __builtin_nan("") : s + (double)b[i];
+            // a mask counts before a NaN, its own or that of the row
+            v[i] = l[i] == minus_inf || b[i] == minus_inf ? -__builtin_inf()
+                   : broken || l[i] != l[i]               ? __builtin_nan("")
+                                                          : s + (double)b[i];
         }
     }
 #pragma unroll

@@ -135,8 +135,8 @@ def route(scores, k, *, score="softmax", bias=None, groups=1, top_groups=1, grou
     s = softmax or sigmoid of the scores; the k experts with the largest s + bias (float32[E]) are chosen, where
     `groups` is given only among the `top_groups` best groups of E / groups experts each (a group counts as its largest
     member, or with "top2" as the sum of its two largest); ties go to the lower index, the choice is that of 64 bits.
-    Weights are scale * s, with `renormalise` divided by the sum of the chosen s.  A score of -inf is never chosen: a
-    slot that finds no expert holds -1, weight 0 and pos -1."""
+    Weights are scale * s, with `renormalise` divided by the sum of the chosen s.  An expert whose score or bias is -inf
+    is never chosen: a slot that finds none holds -1, weight 0 and pos -1."""
     t, device = _first(scores, "scores", 2)
     T, E = scores.shape
     k = operator.index(k)

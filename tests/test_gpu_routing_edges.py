@@ -123,3 +123,24 @@ def test_a_token_does_not_depend_on_its_neighbours(r, dev, score, biased, E, gro
         other = r.route(l[order].to(dev), k, **options)
         assert torch.equal(other.expert, m.expert[order.to(dev)])
         assert torch.equal(other.weight, m.weight[order.to(dev)])
+
+
+@pytest.mark.parametrize("T", [1, 5, 40])
+@pytest.mark.parametrize("E,groups,top_groups,k", [(16, 1, 1, 3), (200, 1, 1, 12), (700, 1, 1, 32)] + LAYOUTS[1:5])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_a_bias_of_minus_infinity_masks_nan(r, dev, T, E, groups, top_groups, k, score):
+    """An expert that its bias masks is never chosen, also where its score, or what the softmax makes of its row, is NaN
+    or infinite."""
+    g = np.random.default_rng(E + T)
+    l = g.normal(size=(T, E)).astype(np.float32)
+    bias = g.normal(size=E).astype(np.float32) * 0.1
+    masked = g.permutation(E)[:E // 3]
+    bias[masked] = -np.inf
+    l[:, masked[0]] = np.nan
+    l[::2, masked[1]] = np.inf
+    m = r.route(torch.from_numpy(l).to(dev), k, score=score, bias=torch.from_numpy(bias).to(dev), groups=groups,
+                top_groups=top_groups, group_score="top2" if groups > 1 else "max")
+    ref = check_choice(m, l, bias, k, score, groups, top_groups, "top2" if groups > 1 else "max")
+    assert not np.isin(ref, masked).any()
+    w = m.weight.cpu().numpy()
+    assert (np.isnan(w[ref >= 0]) if score == "softmax" else np.isfinite(w)).all()
