@@ -738,6 +738,9 @@ int mps_combine_backward(const void *d_dY, const void *d_Z, const float *d_weigh
  * matrix with k = 1):
  *   d_Y[t, :] = d_base[t, :] + d_scale[a] * (d_X[t, :] * d_A[a]^T) * d_B[a]^T
  * and d_Y[t, :] = d_base[t, :] for the tokens behind d_adapter_ptr[E].
+ * The first product, times d_scale, enters the second as a sum of two numbers
+ * of the type: fp16 keeps 22 bits of it (2^-39 of a token's largest at least),
+ * bf16 16.
  * d_base NULL = 0 and may be d_Y; d_scale NULL = 1.  R <= 256, E <= 1024 and
  * T <= MPS_ADAPTERS_MAX_TOKENS, else MPS_ERR_UNSUPPORTED.  Every token has to
  * be in d_row once.  Workspace: mps_adapters_workspace_bytes. */

@@ -90,9 +90,11 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_shrink_kernel(const T *_
 // 64 columns at a time, with the tokens' V in its registers throughout.  V is
 // made in fp32; for the product with B it is split into its rounding to T and
 // the rounding of what that leaves, two instructions instead of one, so that
-// it is not rounded to 8 or 11 bits on the way.  fp16 has no room for values
-// from 65520 on: where a token has one, all of its V are taken down by 2^16
-// and its sums up again.  RANK: the largest rank, in units of 32.
+// it is not rounded to 8 or 11 bits on the way but to 16 (bf16) or 22 (fp16).
+// fp16 has neither room for values from 65520 on nor bits for those below 2^-14:
+// a token's V are multiplied by the power of two that takes the largest of them to
+// 2^14 or more, below 2^15, and its sums divided by it, so that each is kept to
+// 2^-22 of itself or 2^-39 of the largest.  RANK: the largest rank, in units of 32.
 // Row g * 4 + d of the b-th matrix instruction is the column that leaves a lane
 // with 16 bytes of neighbouring columns, and the four lanes of a token with 64.
 template <typename T, int RANK, int MT, bool ALIGNED>
@@ -126,13 +128,13 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
         if ((unsigned)token[m] >= (unsigned)sh.T) token[m] = -1;
     }
     uint4v high[MT][STEPS], low[MT][STEPS];
-    bool taken[MT] = {};  // down by 2^16
+    float back[MT] = {};  // 1 / the factor on a token's V
     if (t.expert >= 0) {
         const float s = scale ? scale[t.expert] : 1.0f;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             float v[STEPS][C];
-            bool far = false;
+            float largest = 0.0f;  // finite one
 #pragma unroll
             for (int step = 0; step < STEPS; ++step) {
                 const int r = step * STEP + g * C;
@@ -153,17 +155,26 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     v[step][c] = r + c < sh.R ? v[step][c] * s : 0.0f;  // infinite rows have NaN behind the rank
-                    far |= __builtin_fabsf(v[step][c]) > 65000.0f;
+                    const float size = __builtin_fabsf(v[step][c]);
+                    if (size < __builtin_inff()) largest = max(largest, size);
                 }
             }
-            // a token's values lie in the four lanes i, i + 16, i + 32, i + 48; its sums come back to the same lanes
-            const bool take = __is_same(T, half_t) && (__ballot(far) >> i & 0x0001000100010001ull) != 0;
+            float factor = 1.0f;
+            back[m] = 1.0f;
+            if constexpr (__is_same(T, half_t)) {
+                // a token's values lie in the four lanes i, i + 16, i + 32, i + 48; its sums come back to the same lanes
+                const auto larger = [](float a, float b) { return max(a, b); };
+                largest = fold<32>(fold<16>(largest, larger), larger);
+                const int up = min(14 + 127 - (int)(float_bits(largest) >> 23), 126);  // -113 .. 126
+                factor = bits_float((unsigned)(127 + up) << 23);
+                back[m] = bits_float((unsigned)(127 - up) << 23);
+            }
 #pragma unroll
             for (int step = 0; step < STEPS; ++step) {
                 T high_of[C], low_of[C];
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    const float x = take ? v[step][c] * 0x1p-16f : v[step][c];
+                    const float x = v[step][c] * factor;
                     high_of[c] = (T)x;
                     const float rest = x - (float)high_of[c];
                     low_of[c] = (T)(__builtin_fabsf(rest) < __builtin_inff() ? rest : 0.0f);  // infinities stand in `high`
@@ -171,7 +182,6 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
                 __builtin_memcpy(&high[m][step], high_of, 16);
                 __builtin_memcpy(&low[m][step], low_of, 16);
             }
-            taken[m] = take;
         }
     }
     const T *b_of = B + (size_t)max(t.expert, 0) * sh.N * sh.R;
@@ -219,7 +229,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             if (token[m] < 0) continue;
-            const float up = __is_same(T, half_t) && taken[m] ? 65536.0f : 1.0f;
+            const float down = __is_same(T, half_t) && t.expert >= 0 ? back[m] : 1.0f;
 #pragma unroll
             for (int b = 0; b < 16 / C; ++b) {
                 const int col = n0 + b * 4 * C + g * C;
@@ -228,7 +238,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
                 float part[C];
 #pragma unroll
                 for (int c = 0; c < C; ++c)
-                    part[c] = __builtin_fmaf(acc[m][b * PER + c / 4][c % 4], up, (float)of_base[c]);
+                    part[c] = __builtin_fmaf(acc[m][b * PER + c / 4][c % 4], down, (float)of_base[c]);
                 store_vec<T, C, ALIGNED>(Y + (size_t)token[m] * sh.N + col, part, sh.N - col);
             }
         }

@@ -144,3 +144,71 @@ def test_a_bias_of_minus_infinity_masks_nan(r, dev, T, E, groups, top_groups, k,
     assert not np.isin(ref, masked).any()
     w = m.weight.cpu().numpy()
     assert (np.isnan(w[ref >= 0]) if score == "softmax" else np.isfinite(w)).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# What stands between the two products of an adapter
+# ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T", [3, 300])
+@pytest.mark.parametrize("R", [4, 16, 40, 130])
+@pytest.mark.parametrize("x,a,b", [(2.0 ** -14, 2.0 ** -6, 2.0 ** 10), (2.0 ** -10, 2.0 ** -14, 2.0 ** 12), (2.0 ** -20, 2.0 ** -12, 2.0 ** 13),
+                                   (1.0, 1.0, 1.0), (2.0 ** 11, 2.0 ** 8, 2.0 ** -10), (2.0 ** 14, 2.0 ** 14, 2.0 ** -14)])
+def test_adapters_fp16_of_any_size(r, dev, T, R, x, a, b):
+    """V = X A^T from far below fp16's smallest numbers to far above its largest, with B that brings it back.  The largest
+    of a token's V is taken to 2^14 or more, so that with two halves each V is off by at most 2^-22 of itself (twice half a
+    step) or by 2^-25 of where the largest is 2^14 (half of the smallest step): 2^-39 of the largest."""
+    t, K, N, E = torch.float16, 64, 48, 2
+    X, A, B = normal(T, T, K, t=t, scale=x / 8), normal(2, E, R, K, t=t, scale=a / 8), normal(3, E, N, R, t=t, scale=b / 4)
+    down = 2.0 ** -8 if x * a * b > 2.0 ** 10 else 1.0  # the results are numbers of fp16
+    B = (B.double() * down).to(t)
+    adapter = torch.arange(T) % E
+    ptr, row, _ = r.columns(adapter.int().view(T, 1).to(dev), E)
+    out = r.adapters_mm(X.to(dev), A.to(dev), B.to(dev), None, ptr, row)
+    V = torch.stack([X[i].double() @ A[adapter[i]].double().t() for i in range(T)])
+    V_size = torch.stack([X[i].double().abs() @ A[adapter[i]].double().abs().t() for i in range(T)])
+    ref, size, split, all_b = (torch.stack([v[i] @ B[adapter[i]].double().abs().t() if v is not V else
+                                            V[i] @ B[adapter[i]].double().t() for i in range(T)])
+                               for v in (V, V_size, V.abs(), torch.ones_like(V)))
+    n = K + R + 4
+    extra = 2.0 ** -22 * split + 2.0 ** -39 * V.abs().amax(1, keepdim=True) * all_b
+    assert ref.abs().max() < 60000
+    close(out, ref, size + extra / ((2 * n + 2) * 2.0 ** -24), n, t)
+
+
+def test_adapters_fp16_large_values_leave_the_others_their_bits(r, dev):
+    """One value of V above fp16's largest, which B multiplies by zero, beside ordinary ones; and values above 2^32 that
+    cancel: the result is finite and exact to 32 bits' sums."""
+    t, K = torch.float16, 32
+    X = torch.zeros(2, K, dtype=t)
+    X[:, 0] = 1.0
+    X[1, 1] = 32768.0
+    A = torch.zeros(1, 4, K, dtype=t)
+    A[0, :, 0] = torch.tensor([0.0, 0.02, 0.3, 0.5])
+    A[0, 0, 1] = 2.125
+    B = torch.tensor([[[0.0, 1.0, 1.0, 1.0]] * 8], dtype=t)
+    ptr, row, _ = r.columns(torch.zeros(2, 1, dtype=torch.int32, device=dev), 1)
+    out = r.adapters_mm(X.to(dev), A.to(dev), B.to(dev), None, ptr, row).cpu()
+    ref = A[0, 1:, 0].double().sum()
+    # V to 2^-39 of 69632 < 2^-22, three of them; then the result's half step of 2^-11
+    assert ((out.double() - ref).abs() <= 2.0 ** -11 * ref + 3 * 2.0 ** -22 + 2.0 ** -22).all()
+    assert torch.equal(out[0], out[1])
+    A[0, 0, 1] = A[0, 1, 1] = 32768.0 * 1.5
+    A[0, :2, 2:] = A[0, 0, 1]
+    X[1, 2:] = 32768.0  # V = 5e10, twice
+    B = torch.tensor([[[1.0, -1.0, 0.0, 0.0]] * 8], dtype=t)
+    A[0, :, 0] = 0.0
+    out = r.adapters_mm(X.to(dev), A.to(dev), B.to(dev), None, ptr, row).cpu()
+    assert (out == 0).all()
+
+
+def test_adapters_fp16_infinite_and_far_values_keep_their_signs(r, dev):
+    """A value that the scale makes infinite beside a finite one of the other sign, far beyond fp16: infinite, not NaN."""
+    t, K = torch.float16, 16
+    X, A = torch.zeros(1, K, dtype=t), torch.zeros(1, 2, K, dtype=t)
+    X[0, 0], X[0, 1] = 32768.0, -2.0 ** -10
+    A[0, 0, 0], A[0, 1, 1] = 1.0, 2.0 ** -10
+    scale = torch.full((1,), 3.0e38)
+    ptr, row, _ = r.columns(torch.zeros(1, 1, dtype=torch.int32, device=dev), 1)
+    out = r.adapters_mm(X.to(dev), A.to(dev), torch.ones(1, 8, 2, dtype=t).to(dev), scale.to(dev), ptr, row).cpu()
+    assert (out == np.inf).all()
