@@ -149,10 +149,12 @@ def route(scores, k, *, score="softmax", bias=None, groups=1, top_groups=1, grou
     _fits(n, E)
     ws, size = _workspace(T, E, k, device) if n > 2048 else (None, 0)  # short ones are known to need none
     if out is None:
-        # one allocation for all that is as long as there are slots, the weights' bits among them
+        # One allocation for all that is as long as there are slots, the weights' bits among them.  `.data`: a version
+        # counter for each, so that an in-place change of the weights is none of the indices that autograd has kept.
         ints = scores.new_empty((4, T, k), dtype=torch.int32)
         expert, weight, slot, pos = ints.unbind()
-        out = Routing(expert, weight.view(torch.float32), scores.new_empty((E + 1,), dtype=torch.int32), slot.view(n), pos)
+        out = Routing(expert.data, weight.view(torch.float32).data, scores.new_empty((E + 1,), dtype=torch.int32),
+                      slot.view(n).data, pos.data)
         at = ints.data_ptr()
         at = at, at + 4 * n, out.expert_ptr.data_ptr(), at + 8 * n, at + 12 * n
     else:

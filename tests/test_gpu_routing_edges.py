@@ -212,3 +212,25 @@ def test_adapters_fp16_infinite_and_far_values_keep_their_signs(r, dev):
     ptr, row, _ = r.columns(torch.zeros(1, 1, dtype=torch.int32, device=dev), 1)
     out = r.adapters_mm(X.to(dev), A.to(dev), torch.ones(1, 8, 2, dtype=t).to(dev), scale.to(dev), ptr, row).cpu()
     assert (out == np.inf).all()
+
+
+def test_parts_of_a_routing_matrix_change_apart(r, dev):
+    """An in-place change of the weights is none of the indices, which autograd may hold for a backward pass."""
+    class Chosen(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, w, expert):
+            ctx.save_for_backward(expert)
+            return w * 2
+
+        @staticmethod
+        def backward(ctx, d):
+            return d * (ctx.saved_tensors[0] >= 0), None
+
+    m = r.route(normal(1, 20, 16).to(dev), 2)
+    before = [x._version for x in m]
+    leaf = torch.ones(20, 2, device=dev, requires_grad=True)
+    out = Chosen.apply(leaf, m.expert)
+    m.weight.mul_(0.5)
+    assert [x._version for x in m] == [before[0], before[1] + 1] + before[2:]
+    out.sum().backward()
+    assert torch.equal(leaf.grad, torch.ones_like(leaf))
