@@ -703,8 +703,10 @@ int mps_route_backward(const void *d_scores, int dtype, const int *d_expert, con
  *   d_Y[p, :] = d_X[row(p), :] * d_W[e]^T  for p in expert e's places.
  * d_slot NULL: row(p) = p and d_X is [M, K].  Else row(p) = d_slot[p] / k and
  * d_X is [M / k, K] (M a multiple of k): the rows of the tokens are gathered
- * as they are needed.  Rows of d_Y from d_expert_ptr[E] on are left as
- * they were. */
+ * as they are needed; a slot out of range counts as a row of zeros.  Rows of
+ * d_Y from d_expert_ptr[E] on are left as they were.  MPS_ERR_UNSUPPORTED where
+ * the tiles are more than a launch holds (2^32 threads, 256 or 512 for a tile of
+ * 16 x 64 elements or more, and at least one tile for an expert). */
 int mps_experts_mm(const void *d_X, const void *d_W, void *d_Y, int dtype, const int *d_expert_ptr, const int *d_slot,
                    int k, int M, int E, int N, int K, void *stream);
 /* Gradient of the rows: d_dX[p, :] = d_dY[p, :] * d_W[e], [M, K] in the order of

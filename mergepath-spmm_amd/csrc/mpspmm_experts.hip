@@ -519,7 +519,7 @@ int launch_stream(const void *A, const void *B, void *out, const int *ptr, const
     sh.col_tiles = ceil_div(WHAT == kForward ? sh.N : sh.K, PP * S);
     sh.row_tiles = ceil_div(sh.N, QP * S);
     const long long others = WHAT == kWeights ? (long long)sh.E * sh.row_tiles : num_row_tiles(sh.M, sh.E, QP * S);
-    if (others * sh.col_tiles > INT_MAX) return MPS_ERR_UNSUPPORTED;
+    if (!fits_launch(others * sh.col_tiles, 64 * WP * WQ)) return MPS_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((experts_stream_kernel<T, WHAT, S, PP, QP, WP, WQ>), dim3((unsigned)(others * sh.col_tiles)),
                        dim3(64 * WP * WQ), 0, st, static_cast<const T *>(A), static_cast<const T *>(B),
                        static_cast<T *>(out), ptr, slot, sh);
@@ -602,7 +602,7 @@ int launch_few(const void *X, const void *W, void *Y, const int *ptr, const int 
 {
     sh.col_tiles = ceil_div(sh.N, 16 * kFewColumns);
     const long long blocks = num_row_tiles(sh.M, sh.E, 16 * MT) * sh.col_tiles;
-    if (blocks > INT_MAX) return MPS_ERR_UNSUPPORTED;
+    if (!fits_launch(blocks, 64 * kFewWaves)) return MPS_ERR_UNSUPPORTED;
 #define MPS_LAUNCH_FEW(ALIGNED)                                                                                       \
     hipLaunchKernelGGL((experts_few_kernel<T, MT, ALIGNED>), dim3((unsigned)blocks), dim3(64 * kFewWaves), 0, st,     \
                        static_cast<const T *>(X), static_cast<const T *>(W), static_cast<T *>(Y), ptr, slot, sh)
@@ -620,7 +620,7 @@ int launch_tile(const void *A, const void *B, void *out, const int *ptr, const i
     sh.col_tiles = ceil_div(WHAT == kForward ? sh.N : sh.K, S);
     sh.row_tiles = ceil_div(sh.N, S);
     const long long others = WHAT == kWeights ? (long long)sh.E * sh.row_tiles : num_row_tiles(sh.M, sh.E, S);
-    if (others * sh.col_tiles > INT_MAX) return MPS_ERR_UNSUPPORTED;
+    if (!fits_launch(others * sh.col_tiles, kThreads)) return MPS_ERR_UNSUPPORTED;
 #define MPS_LAUNCH_TILE(ALIGNED)                                                                                 \
     hipLaunchKernelGGL((experts_tile_kernel<T, WHAT, S, ALIGNED>), dim3((unsigned)(others * sh.col_tiles)),      \
                        dim3(kThreads), 0, st, static_cast<const T *>(A), static_cast<const T *>(B),              \

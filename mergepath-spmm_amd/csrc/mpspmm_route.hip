@@ -502,7 +502,7 @@ __global__ __launch_bounds__(kRouteBlock) void route_kernel(const T *__restrict_
 {
     extern __shared__ unsigned long long route_lds[];
     const int lane = threadIdx.x & (L - 1), in_block = threadIdx.x / L;
-    const long long t = (long long)blockIdx.x * (kRouteBlock / L) + in_block;
+    const long long t = block_number() * (kRouteBlock / L) + in_block;
     const bool live = t < sh.T;
     int e;
     float w;
@@ -747,7 +747,7 @@ __global__ __launch_bounds__(kRouteBlock) void route_backward_kernel(const T *__
                                                                      T *__restrict__ dscores)
 {
     const int lane = threadIdx.x & 63;
-    const long long t = (long long)blockIdx.x * (kRouteBlock / 64) + (threadIdx.x >> 6);
+    const long long t = block_number() * (kRouteBlock / 64) + (threadIdx.x >> 6);
     if (t >= sh.T) return;
     const T *row = scores + t * sh.E;
     T *out = dscores + t * sh.E;
@@ -816,7 +816,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const T *__restrict__ Z, c
                                                       int k, int M, int N, int per_row)
 {
     constexpr int V = 16 / sizeof(T);
-    const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long item = block_number() * 256 + threadIdx.x;
     const long long t = item / per_row;
     if (t >= T_) return;
     const int col = (int)(item - t * per_row) * V;
@@ -862,7 +862,7 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T *__restri
 {
     constexpr int V = 16 / sizeof(T);
     const int lane = threadIdx.x & (L - 1);
-    const long long at = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const long long at = block_number() * (256 / L) + threadIdx.x / L;
     if (at >= M) return;
     const int p = (int)at;
     const int s = slot[p];
@@ -972,7 +972,7 @@ int launch_route(const T *scores, const float *bias, RouteShape sh, int *expert,
     return with_route_lanes(sh, [&](auto ipl, auto lanes) -> int {
         constexpr int IPL = decltype(ipl)::value, L = decltype(lanes)::value;
         fit_groups(IPL);
-        hipLaunchKernelGGL((route_kernel<T, IPL, L>), dim3(ceil_div(sh.T, kRouteBlock / L)), dim3(kRouteBlock),
+        hipLaunchKernelGGL((route_kernel<T, IPL, L>), grid_of(ceil_div(sh.T, kRouteBlock / L)), dim3(kRouteBlock),
                            per_token * (kRouteBlock / L), st, scores, bias, sh, expert, weight);
         MPS_HIP_TRY(hipGetLastError());
         return MPS_OK;
@@ -988,7 +988,7 @@ int launch_combine(const void *Z, const int *pos, const float *weight, const voi
     if (blocks > INT_MAX) return MPS_ERR_UNSUPPORTED;
     const bool fast = rows_of_16(Z, N, sizeof(T)) && rows_of_16(Y, N, sizeof(T)) && rows_of_16(base, N, sizeof(T));
 #define MPS_LAUNCH_COMBINE(ALIGNED)                                                                               \
-    hipLaunchKernelGGL((combine_kernel<T, ALIGNED>), dim3((unsigned)blocks), dim3(256), 0, st,                    \
+    hipLaunchKernelGGL((combine_kernel<T, ALIGNED>), grid_of(blocks), dim3(256), 0, st,                           \
                        static_cast<const T *>(Z), pos, weight, static_cast<const T *>(base), static_cast<T *>(Y), \
                        T_, k, M, N, per_row)
     if (fast) MPS_LAUNCH_COMBINE(true);
@@ -1006,7 +1006,7 @@ int launch_combine_backward(const void *dY, const void *Z, const float *weight, 
     // as many lanes as a row has chunks (34076 places of 39 columns bf16: 10.6 us a call, 29.7 with 64)
     const int chunks = ceil_div(N, 16 / (int)sizeof(T));
 #define MPS_LAUNCH_COMBINE(L, ALIGNED)                                                                             \
-    hipLaunchKernelGGL((combine_backward_kernel<T, L, ALIGNED>), dim3(ceil_div(M, 256 / L)), dim3(256), 0, st,     \
+    hipLaunchKernelGGL((combine_backward_kernel<T, L, ALIGNED>), grid_of(ceil_div(M, 256 / L)), dim3(256), 0, st,  \
                        static_cast<const T *>(dY), static_cast<const T *>(Z), weight, expert_ptr, E, slot,         \
                        static_cast<T *>(dZ), dweight, k, M, N)
 #define MPS_LAUNCH_LANES(L)                     \
@@ -1096,7 +1096,7 @@ int mps_route_backward(const void *d_scores, int dtype, const int *d_expert, con
     RouteShape sh = make_shape(*options, T, E);
     hipStream_t st = static_cast<hipStream_t>(stream);
 #define MPS_LAUNCH_BACKWARD(TYPE)                                                                                  \
-    hipLaunchKernelGGL((route_backward_kernel<TYPE>), dim3(ceil_div(T, kRouteBlock / 64)), dim3(kRouteBlock), 0, st, \
+    hipLaunchKernelGGL((route_backward_kernel<TYPE>), grid_of(ceil_div(T, kRouteBlock / 64)), dim3(kRouteBlock), 0, st, \
                        static_cast<const TYPE *>(d_scores), d_expert, d_dweight, sh, static_cast<TYPE *>(d_dscores))
     if (dtype == MPS_F32) MPS_LAUNCH_BACKWARD(float);
     else if (dtype == MPS_F16) MPS_LAUNCH_BACKWARD(half_t);

@@ -30,6 +30,19 @@ inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintp
 
 inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
+// A launch holds fewer than 2^32 threads in a dimension, which a wavefront for
+// every one of 2^26 tokens reaches; of more only the rest is run, without an
+// error.  More workgroups than kGridRow go into rows of a second dimension.  Numbers from `blocks` on occur; a kernel gives them nothing.
+constexpr int kGridRow = 1 << 22;
+inline dim3 grid_of(long long blocks)
+{
+    return blocks <= kGridRow ? dim3((unsigned)blocks) : dim3(kGridRow, (unsigned)ceil_div(blocks, kGridRow));
+}
+__device__ __forceinline__ long long block_number() { return (long long)blockIdx.y * kGridRow + blockIdx.x; }
+
+// Whether so many workgroups fit one dimension.
+inline bool fits_launch(long long blocks, int threads) { return blocks <= 0xFFFFFFFFll / threads; }
+
 // A matrix whose rows are loaded 16 bytes at a time: aligned base, rows of whole 16 bytes.
 inline bool rows_of_16(const void *p, long long row_elems, int elem_bytes)
 {

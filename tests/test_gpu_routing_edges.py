@@ -234,3 +234,82 @@ def test_parts_of_a_routing_matrix_change_apart(r, dev):
     assert [x._version for x in m] == [before[0], before[1] + 1] + before[2:]
     out.sum().backward()
     assert torch.equal(leaf.grad, torch.ones_like(leaf))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# More rows than one dimension of a launch has threads
+# ---------------------------------------------------------------------------------------------------------------------
+
+def test_route_backward_of_many_tokens(r, dev):
+    """2^26 tokens and some, a wavefront each: 2^32 threads."""
+    T, E = (1 << 26) + 77, 2
+    scores = torch.zeros(T, E, dtype=torch.float16, device=dev)
+    expert = torch.zeros(T, 1, dtype=torch.int32, device=dev)
+    dweight = torch.zeros(T, 1, device=dev)
+    for first in (0, 1 << 25, T - 1000):
+        scores[first:first + 900] = normal(first, 900, E, t=torch.float16).to(dev)
+        expert[first:first + 900:2] = 1
+        dweight[first:first + 900] = normal(first + 1, 900, 1).to(dev)
+    out = r.route_backward(scores, expert, dweight)
+    for at in (slice(0, 1000), slice(1 << 25, (1 << 25) + 1000), slice(T - 1000, T)):
+        x = scores[at].cpu().double().requires_grad_()
+        dw = dweight[at].cpu().double()
+        weights_of(x, expert[at].cpu(), "softmax", False, 1.0).backward(dw)
+        close(out[at], x.grad, 2 * dw.abs().expand(-1, E), 16, torch.float16)
+
+
+def test_route_of_many_tokens(r, dev):
+    """2^28 tokens and some, 16 lanes each."""
+    T, E = (1 << 28) + 77, 3
+    scores = torch.zeros(T, E, dtype=torch.bfloat16, device=dev)
+    scores[:, 2] = 1.0
+    scores[-77:, 1] = 2.0
+    scores[:50, 0] = 3.0
+    m = r.route(scores, 1, score="sigmoid")
+    assert m.expert_ptr.cpu().tolist() == [0, 50, 127, T]
+    assert (m.expert[:50] == 0).all() and (m.expert[50:-77] == 2).all() and (m.expert[-77:] == 1).all()
+    assert torch.equal(m.slot[:50].cpu(), torch.arange(50, dtype=torch.int32))
+    assert torch.equal(m.slot[50:127].cpu(), torch.arange(T - 77, T, dtype=torch.int32))
+    assert torch.equal(m.pos[-77:, 0].cpu(), torch.arange(50, 127, dtype=torch.int32))
+    assert int(m.pos[T - 78, 0]) == T - 1
+    one = (1.0 / (1.0 + np.exp(-1.0)))
+    assert (m.weight[50:-77] - one).abs().max() <= 2.0 ** -19
+
+
+def test_combine_backward_of_many_places(r, dev):
+    """2^29 places and some, 8 lanes each."""
+    k = 32
+    T = (1 << 24) + 3
+    M, t = T * k, torch.bfloat16
+    g = torch.Generator(device=dev).manual_seed(1)
+    dY = torch.randint(-8, 9, (T, 1), generator=g, device=dev).to(t)
+    Z = torch.randint(-8, 9, (M, 1), generator=g, device=dev, dtype=torch.int8).to(t)
+    weight = torch.full((T, k), 0.5, device=dev)
+    ptr = torch.tensor([0, M - 5], dtype=torch.int32, device=dev)
+    slot = torch.arange(M, dtype=torch.int32, device=dev).flip(0)
+    got = r.combine_backward(dY, Z, weight, ptr, slot)
+    del weight, slot
+    rows = dY.view(T, 1).expand(T, k).reshape(M)  # of every slot
+    want = (rows * Z.view(M).flip(0)).float()     # whole numbers below 2^7
+    want[:5] = 0.0
+    assert torch.equal(got["dweight"].view(M), want)
+    want = (rows * 0.5).flip(0)
+    want[-5:] = 0.0
+    assert torch.equal(got["dZ"].view(M), want)
+
+
+def test_combine_of_many_rows(r, dev):
+    """More than 2^32 chunks of 16 bytes in the result."""
+    N, t = 1024, torch.float16
+    T = (1 << 25) + 9
+    if torch.cuda.mem_get_info(dev)[0] < 100 << 30:
+        torch.cuda.empty_cache()
+    Z = normal(1, 40, N, t=t).to(dev)
+    pos = (torch.arange(T, device=dev) % 41).int().view(T, 1)
+    pos[pos == 40] = -1
+    out = r.combine(Z, pos)
+    for at in (slice(0, 300), slice(T // 2, T // 2 + 300), slice(T - 300, T)):
+        p = pos[at, 0].long()
+        assert torch.equal(out[at], torch.where((p < 0)[:, None], torch.zeros((), dtype=t, device=dev), Z[p.clamp(min=0)]))
+    del out
+    torch.cuda.empty_cache()

@@ -151,3 +151,12 @@ def test_route_options_are_values(pkg):
     for bad in (dict(k=2.5), dict(groups="2"), dict(scale="x"), dict(scale=None)):
         with pytest.raises((TypeError, ValueError)):
             of(**bad)
+
+
+def test_experts_of_more_tiles_than_a_launch_holds(L):
+    for fn in (L.mps_experts_mm, L.mps_experts_mm_dw):
+        assert fn(P, P, P, 1, P, None, 1, 64, 1 << 24, 1, 1, None) == UNSUPPORTED
+        assert fn(P, P, P, 0, P, None, 1, 1 << 20, 1 << 22, 1000, 8, None) == UNSUPPORTED
+    assert L.mps_experts_mm(P, P, P, 2, P, None, 1, 1 << 30, 1 << 10, 1 << 20, 8, None) == UNSUPPORTED
+    assert L.mps_experts_mm_dx(P, P, P, 1, P, 64, 1 << 24, 1, 1, None) == UNSUPPORTED
+    assert L.mps_experts_mm(P, P, P, 1, P, None, 1, 64, 2 ** 31 - 1, 1, 1, None) == UNSUPPORTED
