@@ -313,3 +313,127 @@ def test_combine_of_many_rows(r, dev):
         assert torch.equal(out[at], torch.where((p < 0)[:, None], torch.zeros((), dtype=t, device=dev), Z[p.clamp(min=0)]))
     del out
     torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# The shapes of the experts' products
+# ---------------------------------------------------------------------------------------------------------------------
+
+def ragged(mean, E, seed):
+    """Rows of E experts with the given mean exactly, uneven, one expert without rows where there are more than two."""
+    g = np.random.default_rng(seed)
+    share = g.random(E) + 0.1
+    if E > 2:
+        share[E // 2] = 0.0
+    counts = np.floor(share / share.sum() * mean * E).astype(int)
+    counts[0] += mean * E - counts.sum()
+    return counts.tolist()
+
+
+# Every shape of the three products by the rows of an expert, the number of tiles and the rows' alignment (whole 16 bytes
+# or not): few rows, 64 and 128 wide through registers and straight into LDS, 256 x 256.
+SHAPES = [  # mean rows, experts, k, N, K
+    (8, 5, 4, 96, 200),          # 16 rows a tile
+    (24, 5, 3, 80, 136),         # 32 rows a tile
+    (25, 6, 5, 200, 264),        # 64 wide
+    (150, 4, 2, 333, 203),       # 64 wide, odd rows
+    (40, 64, 4, 640, 1032),      # 128 wide, all three products: 512 tiles and more
+    (40, 64, 4, 645, 1031),      # the same, odd rows
+    (384, 3, 3, 320, 568),       # 256 x 256 for 16 bits: several experts, several tiles of columns
+    (500, 4, 5, 264, 1032),
+    (500, 4, 5, 261, 1027),
+]
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_experts_shapes(r, dev, t, gather, shape):
+    mean, E, k, N, K = SHAPES[shape]
+    counts = ragged(mean, E, shape)
+    ptr, M = segments(counts, 0)
+    assert M == mean * E and M % k == 0
+    t = TYPES[t]
+    slot = shuffled_slots(M, 9)
+    X = normal(1, M // k if gather else M, K, t=t)
+    W, dY = normal(2, E, N, K, t=t, scale=K ** -0.5), normal(3, M, N, t=t)
+    x, w, dy, p = X.to(dev), W.to(dev), dY.to(dev), ptr.to(dev)
+    how = dict(slot=slot.to(dev), k=k) if gather else {}
+    Y, dW = r.experts_mm(x, w, p, **how), r.experts_mm_dw(dy, x, p, **how)
+    dX = None if gather else r.experts_mm_dx(dy, w, p)
+    rows = X.double()[slot.long() // k] if gather else X.double()
+    W, dY = W.double(), dY.double()
+    for e in range(E):
+        a = slice(int(ptr[e]), int(ptr[e + 1]))
+        if counts[e]:
+            close(Y[a], rows[a] @ W[e].t(), rows[a].abs() @ W[e].abs().t(), K, t)
+            if not gather:
+                close(dX[a], dY[a] @ W[e], dY[a].abs() @ W[e].abs(), N, t)
+        close(dW[e], dY[a].t() @ rows[a], dY[a].abs().t() @ rows[a].abs(), counts[e], t)
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("counts", [[0, 0, 1000, 0, 0, 0, 0, 0, 0, 0] * 12, [700] + [0] * 99, [1] * 99 + [301]])
+def test_experts_of_uneven_length(r, dev, t, counts):
+    """One expert with nearly all rows, at means that choose the kernels for few rows."""
+    t = TYPES[t]
+    E, N, K = len(counts), 72, 96
+    ptr, M = segments(counts)
+    X, W, dY = normal(1, M, K, t=t), normal(2, E, N, K, t=t, scale=0.1), normal(3, M, N, t=t)
+    x, w, dy, p = X.to(dev), W.to(dev), dY.to(dev), ptr.to(dev)
+    Y, dX, dW = r.experts_mm(x, w, p), r.experts_mm_dx(dy, w, p), r.experts_mm_dw(dy, x, p).cpu()
+    X, W, dY = X.double(), W.double(), dY.double()
+    for e in range(E):
+        a = slice(int(ptr[e]), int(ptr[e + 1]))
+        if counts[e]:
+            close(Y[a], X[a] @ W[e].t(), X[a].abs() @ W[e].abs().t(), K, t)
+            close(dX[a], dY[a] @ W[e], dY[a].abs() @ W[e].abs(), N, t)
+            close(dW[e], dY[a].t() @ X[a], dY[a].abs().t() @ X[a].abs(), counts[e], t)
+        else:
+            assert (dW[e] == 0).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# The gradient of the scores
+# ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalise", [False, True])
+@pytest.mark.parametrize("E,k", [(8, 3), (72, 6), (300, 32)])
+def test_route_backward_of_masked_scores(r, dev, score, renormalise, E, k):
+    """Rows with some scores, all but one and all of them -inf: their gradient is zero, and nothing is NaN."""
+    T = 40
+    l = normal(1, T, E, scale=1.5)
+    l[torch.rand(T, E, generator=gen(2)) < 0.6] = -np.inf
+    l[3], l[4] = -np.inf, -np.inf
+    l[4, E // 2] = 0.25
+    m = r.route(l.to(dev), k, score=score, renormalise=renormalise, scale=2.5)
+    expert, dw = m.expert.cpu(), normal(3, T, k)
+    assert (expert[3] == -1).all() and expert[4].tolist() == [E // 2] + [-1] * (k - 1)
+    got = r.route_backward(l.to(dev), m.expert, dw.to(dev), score=score, renormalise=renormalise, scale=2.5)
+    x = l.double().clamp(min=-1e4).requires_grad_()  # exp(-1e4) is zero in 64 bits too, and its derivative
+    weights_of(x, expert, score, renormalise, 2.5).backward(dw.double())
+    ref = x.grad
+    ref[l == -np.inf] = 0.0
+    close(got, ref, 2 * 2.5 * dw.double().abs().amax(1, keepdim=True).expand(T, E), 16, torch.float32)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalise", [False, True])
+def test_route_backward_against_differences_of_the_kernel(r, dev, score, renormalise):
+    """The gradient along a direction against the difference of the weights that the forward kernel itself gives a step
+    of h = 2^-7 to each side, where it makes the same choice.  With |v| <= 2 the third derivative of a share w of one is
+    below 170 w (powers and moments of numbers that differ by at most 4: 64 + 48 + 8, and 50 for the curvature of the
+    sigmoid's logarithm), and that of a sigmoid below 1; with |dw| <= 4 and shares that add up to one: 4 * 170 h^2 / 6 <
+    0.007.  The weights' own 2^-19: 6 * 4 * 2^-19 / h < 0.006; the scores' rounding to 2^-22 less than 0.001."""
+    T, E, k = 40, 48, 6
+    l = normal(5, T, E)
+    dw = normal(6, T, k).clamp(-4, 4)
+    v = normal(7, T, E).clamp(-2, 2)
+    h = 2.0 ** -7
+    m, up, down = (r.route((l + d * v).to(dev), k, score=score, renormalise=renormalise) for d in (0.0, h, -h))
+    grad = r.route_backward(l.to(dev), m.expert, dw.to(dev), score=score, renormalise=renormalise).cpu().double()
+    same = ((up.expert == m.expert) & (down.expert == m.expert)).all(1).cpu()
+    assert same.sum() >= T // 4
+    slope = ((up.weight.cpu().double() - down.weight.cpu().double()) * dw.double()).sum(1) / (2 * h)
+    assert ((grad * v.double()).sum(1) - slope)[same].abs().max() < 0.014
