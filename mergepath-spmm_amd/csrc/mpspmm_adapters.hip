@@ -24,7 +24,7 @@ struct AdaptersShape {
 // of 16 MT tokens and part; its four wavefronts take 128 bytes of a row in turn
 // and add up through LDS.  A step of 64 bytes loads MT + RT chunks for MT * RT
 // matrix instructions.
-template <typename T, int RT, int MT, bool ALIGNED>
+template <typename T, int RT, int MT>
 __global__ __launch_bounds__(64 * kWaves) void adapters_shrink_kernel(const T *__restrict__ X, const T *__restrict__ A,
                                                                       const int *__restrict__ ptr,
                                                                       const int *__restrict__ row_of,
@@ -58,9 +58,9 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_shrink_kernel(const T *_
             const int k = base + half * STEP + g * C;
             uint4v q[MT], p[RT];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) q[m] = load_chunk<T, ALIGNED>(x[m] + k, live[m] ? k1 - k : 0);
+            for (int m = 0; m < MT; ++m) q[m] = load_chunk<T>(x[m] + k, live[m] ? k1 - k : 0);
 #pragma unroll
-            for (int n = 0; n < RT; ++n) p[n] = load_chunk<T, ALIGNED>(a[n] + k, n * 16 + i < sh.R ? k1 - k : 0);
+            for (int n = 0; n < RT; ++n) p[n] = load_chunk<T>(a[n] + k, n * 16 + i < sh.R ? k1 - k : 0);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_shrink_kernel(const T *_
 // 2^-22 of itself or 2^-39 of the largest.  RANK: the largest rank, in units of 32.
 // Row g * 4 + d of the b-th matrix instruction is the column that leaves a lane
 // with 16 bytes of neighbouring columns, and the four lanes of a token with 64.
-template <typename T, int RANK, int MT, bool ALIGNED>
+template <typename T, int RANK, int MT>
 __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const float *__restrict__ V,
                                                                       const T *__restrict__ B,
                                                                       const float *__restrict__ scale, const T *base,
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
 #pragma unroll
             for (int b = 0; b < 16 / C; ++b) {
                 const int col = n0 + b * 4 * C + g * C;
-                o.y[m][b] = load_chunk<T, ALIGNED>(base + (base && token[m] >= 0 ? (size_t)token[m] * sh.N + col : 0),
+                o.y[m][b] = load_chunk<T>(base + (base && token[m] >= 0 ? (size_t)token[m] * sh.N + col : 0),
                                                    base && token[m] >= 0 ? sh.N - col : 0);
             }
         if (t.expert < 0) return;
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const int col = n0 + b / PER * 4 * C + (i >> 2) * C + b % PER * 4 + (i & 3);
-                o.p[step][b] = load_chunk<T, ALIGNED>(b_of + (size_t)(col < sh.N ? col : 0) * sh.R + r,
+                o.p[step][b] = load_chunk<T>(b_of + (size_t)(col < sh.N ? col : 0) * sh.R + r,
                                                       col < sh.N ? sh.R - r : 0);
             }
         }
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
 #pragma unroll
                 for (int c = 0; c < C; ++c)
                     part[c] = __builtin_fmaf(acc[m][b * PER + c / 4][c % 4], down, (float)of_base[c]);
-                store_vec<T, C, ALIGNED>(Y + (size_t)token[m] * sh.N + col, part, sh.N - col);
+                store_vec<T, C>(Y + (size_t)token[m] * sh.N + col, part, sh.N - col);
             }
         }
     };
@@ -285,10 +285,7 @@ int launch_shrink(const T *X, const T *A, const int *ptr, const int *row_of, flo
                   hipStream_t st)
 {
     const dim3 grid((unsigned)num_row_tiles(sh.T, sh.E, 16 * MT), sh.splits);
-    if (rows_of_16(X, sh.K, sizeof(T)) && rows_of_16(A, sh.K, sizeof(T)))
-        hipLaunchKernelGGL((adapters_shrink_kernel<T, RT, MT, true>), grid, dim3(64 * kWaves), 0, st, X, A, ptr, row_of, V, sh);
-    else
-        hipLaunchKernelGGL((adapters_shrink_kernel<T, RT, MT, false>), grid, dim3(64 * kWaves), 0, st, X, A, ptr, row_of, V, sh);
+    hipLaunchKernelGGL((adapters_shrink_kernel<T, RT, MT>), grid, dim3(64 * kWaves), 0, st, X, A, ptr, row_of, V, sh);
     MPS_HIP_TRY(hipGetLastError());
     return MPS_OK;
 }
@@ -302,13 +299,8 @@ int launch_expand(const float *V, const T *B, const float *scale, const T *base,
     long long columns = (long long)sh.N * tiles / 1024 / 256 * 256;
     columns = columns < 256 || RANK > 2 ? 256 : columns > 1024 ? 1024 : columns;
     const dim3 grid(ceil_div(sh.N, columns), (unsigned)tiles);
-    const bool fast = rows_of_16(B, sh.R, sizeof(T)) && rows_of_16(base, sh.N, sizeof(T)) && rows_of_16(Y, sh.N, sizeof(T));
-    if (fast)
-        hipLaunchKernelGGL((adapters_expand_kernel<T, RANK, MT, true>), grid, dim3(64 * kWaves), 0, st, V, B, scale, base,
-                           Y, ptr, row_of, (int)columns, sh);
-    else
-        hipLaunchKernelGGL((adapters_expand_kernel<T, RANK, MT, false>), grid, dim3(64 * kWaves), 0, st, V, B, scale, base,
-                           Y, ptr, row_of, (int)columns, sh);
+    hipLaunchKernelGGL((adapters_expand_kernel<T, RANK, MT>), grid, dim3(64 * kWaves), 0, st, V, B, scale, base, Y, ptr,
+                       row_of, (int)columns, sh);
     MPS_HIP_TRY(hipGetLastError());
     return MPS_OK;
 }

@@ -111,7 +111,7 @@ __device__ __forceinline__ unsigned token_of(unsigned slot, const ExpertsShape &
 
 enum Product { kForward, kRows, kWeights };
 
-template <typename T, Product WHAT, int S, bool ALIGNED>
+template <typename T, Product WHAT, int S>
 __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__restrict__ A, const T *__restrict__ B,
                                                                    T *__restrict__ out, const int *__restrict__ ptr,
                                                                    const int *__restrict__ slot, ExpertsShape sh)
@@ -195,18 +195,18 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
                         }
                     }
                 }
-                p_hold[n] = load_chunk<T, ALIGNED>(p_src[n] + (from < 0 ? 0 : from * sh.K), from < 0 ? 0 : p_valid[n]);
+                p_hold[n] = load_chunk<T>(p_src[n] + (from < 0 ? 0 : from * sh.K), from < 0 ? 0 : p_valid[n]);
             } else {
                 const int r = r0 + id % 8 * V;
-                p_hold[n] = load_chunk<T, ALIGNED>(p_src[n] + r, p_src[n] ? depth - r : 0);
+                p_hold[n] = load_chunk<T>(p_src[n] + r, p_src[n] ? depth - r : 0);
             }
             if constexpr (QT) {
                 const int r = r0 + id / ROW;
-                q_hold[n] = load_chunk<T, ALIGNED>(q_src[n] + (size_t)(first + (r < depth ? r : 0)) * sh.N,
+                q_hold[n] = load_chunk<T>(q_src[n] + (size_t)(first + (r < depth ? r : 0)) * sh.N,
                                                    r < depth ? q_valid[n] : 0);
             } else {
                 const int r = r0 + id % 8 * V;
-                q_hold[n] = load_chunk<T, ALIGNED>(q_src[n] + r, q_src[n] ? depth - r : 0);
+                q_hold[n] = load_chunk<T>(q_src[n] + r, q_src[n] ? depth - r : 0);
             }
         }
     };
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
         for (int b = 0; b < F; ++b) {
             const int p = col0 + p_base + 16 * b + (lane >> 4) * 4;
             const float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
-            if (p < cols) store_vec<T, 4, ALIGNED>(row + p, v, cols - p);
+            if (p < cols) store_vec<T, 4>(row + p, v, cols - p);
         }
     }
 }
@@ -508,7 +508,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void experts_stream_kernel(const T
         for (int b = 0; b < FP; ++b) {
             const int p = col0 + p_base + 16 * b + (lane >> 4) * 4;
             const float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
-            if (p < cols) store_vec<T, 4, true>(row + p, v, cols - p);
+            if (p < cols) store_vec<T, 4>(row + p, v, cols - p);
         }
     }
 }
@@ -534,7 +534,7 @@ int launch_stream(const void *A, const void *B, void *out, const int *ptr, const
 // LDS.  No barrier until the end, so that many loads are on their way.
 constexpr int kFewWaves = 4, kFewColumns = 4;  // in 16s
 
-template <typename T, int MT, bool ALIGNED>
+template <typename T, int MT>
 __global__ __launch_bounds__(64 * kFewWaves) void experts_few_kernel(const T *__restrict__ X, const T *__restrict__ W,
                                                                      T *__restrict__ Y, const int *__restrict__ ptr,
                                                                      const int *__restrict__ slot, ExpertsShape sh)
@@ -567,9 +567,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void experts_few_kernel(const T *__
         for (int half = 0; half < 2; ++half) {
             const int k = base + half * STEP + g * C;
 #pragma unroll
-            for (int n = 0; n < RT; ++n) p[half][n] = load_chunk<T, ALIGNED>(w[n] + k, sh.K - k);
+            for (int n = 0; n < RT; ++n) p[half][n] = load_chunk<T>(w[n] + k, sh.K - k);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) q[half][m] = load_chunk<T, ALIGNED>(x[m] + k, live[m] ? sh.K - k : 0);
+            for (int m = 0; m < MT; ++m) q[half][m] = load_chunk<T>(x[m] + k, live[m] ? sh.K - k : 0);
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half)
@@ -590,44 +590,33 @@ __global__ __launch_bounds__(64 * kFewWaves) void experts_few_kernel(const T *__
 #pragma unroll
             for (int other = 1; other < kFewWaves; ++other) sum += join[other][wave][lane];
             const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-            store_vec<T, 4, ALIGNED>(Y + (size_t)(t.first + 16 * m + i) * sh.N + col, v, sh.N - col);
+            store_vec<T, 4>(Y + (size_t)(t.first + 16 * m + i) * sh.N + col, v, sh.N - col);
         }
     }
 }
 static_assert(kFewColumns == kFewWaves, "a wavefront adds up 16 columns");
 
 template <typename T, int MT>
-int launch_few(const void *X, const void *W, void *Y, const int *ptr, const int *slot, ExpertsShape sh, bool fast,
-               hipStream_t st)
+int launch_few(const void *X, const void *W, void *Y, const int *ptr, const int *slot, ExpertsShape sh, hipStream_t st)
 {
     sh.col_tiles = ceil_div(sh.N, 16 * kFewColumns);
     const long long blocks = num_row_tiles(sh.M, sh.E, 16 * MT) * sh.col_tiles;
     if (!fits_launch(blocks, 64 * kFewWaves)) return MPS_ERR_UNSUPPORTED;
-#define MPS_LAUNCH_FEW(ALIGNED)                                                                                       \
-    hipLaunchKernelGGL((experts_few_kernel<T, MT, ALIGNED>), dim3((unsigned)blocks), dim3(64 * kFewWaves), 0, st,     \
-                       static_cast<const T *>(X), static_cast<const T *>(W), static_cast<T *>(Y), ptr, slot, sh)
-    if (fast) MPS_LAUNCH_FEW(true);
-    else MPS_LAUNCH_FEW(false);
-#undef MPS_LAUNCH_FEW
+    hipLaunchKernelGGL((experts_few_kernel<T, MT>), dim3((unsigned)blocks), dim3(64 * kFewWaves), 0, st,
+                       static_cast<const T *>(X), static_cast<const T *>(W), static_cast<T *>(Y), ptr, slot, sh);
     MPS_HIP_TRY(hipGetLastError());
     return MPS_OK;
 }
 
 template <typename T, Product WHAT, int S>
-int launch_tile(const void *A, const void *B, void *out, const int *ptr, const int *slot, ExpertsShape sh, bool fast,
-                hipStream_t st)
+int launch_tile(const void *A, const void *B, void *out, const int *ptr, const int *slot, ExpertsShape sh, hipStream_t st)
 {
     sh.col_tiles = ceil_div(WHAT == kForward ? sh.N : sh.K, S);
     sh.row_tiles = ceil_div(sh.N, S);
     const long long others = WHAT == kWeights ? (long long)sh.E * sh.row_tiles : num_row_tiles(sh.M, sh.E, S);
     if (!fits_launch(others * sh.col_tiles, kThreads)) return MPS_ERR_UNSUPPORTED;
-#define MPS_LAUNCH_TILE(ALIGNED)                                                                                 \
-    hipLaunchKernelGGL((experts_tile_kernel<T, WHAT, S, ALIGNED>), dim3((unsigned)(others * sh.col_tiles)),      \
-                       dim3(kThreads), 0, st, static_cast<const T *>(A), static_cast<const T *>(B),              \
-                       static_cast<T *>(out), ptr, slot, sh)
-    if (fast) MPS_LAUNCH_TILE(true);
-    else MPS_LAUNCH_TILE(false);
-#undef MPS_LAUNCH_TILE
+    hipLaunchKernelGGL((experts_tile_kernel<T, WHAT, S>), dim3((unsigned)(others * sh.col_tiles)), dim3(kThreads), 0, st,
+                       static_cast<const T *>(A), static_cast<const T *>(B), static_cast<T *>(out), ptr, slot, sh);
     MPS_HIP_TRY(hipGetLastError());
     return MPS_OK;
 }
@@ -644,8 +633,8 @@ int launch_experts(const void *A, const void *B, void *out, const int *ptr, cons
     if constexpr (WHAT == kForward) {
         // Few rows an expert: the tiles below would be nearly empty and their workgroups few (32 tokens, 6 of 64 experts,
         // 2048 x 1024 bf16: 59 us, 62 - 80 with tiles of 128).
-        if (M <= 8LL * E) return launch_few<T, 1>(A, B, out, ptr, slot, sh, fast, st);
-        if (M <= 24LL * E) return launch_few<T, 2>(A, B, out, ptr, slot, sh, fast, st);
+        if (M <= 8LL * E) return launch_few<T, 1>(A, B, out, ptr, slot, sh, st);
+        if (M <= 24LL * E) return launch_few<T, 2>(A, B, out, ptr, slot, sh, st);
     }
     // Tiles of 64 where tiles of 128 would leave compute units without one.
     const long long tiles = WHAT == kWeights ? (long long)E * ceil_div(N, 128) * ceil_div(K, 128)
@@ -662,8 +651,8 @@ int launch_experts(const void *A, const void *B, void *out, const int *ptr, cons
         return small ? launch_stream<T, WHAT, 64, 1, 1, 2, 2>(A, B, out, ptr, slot, sh, st)
                      : launch_stream<T, WHAT, 128, 1, 1, 2, 2>(A, B, out, ptr, slot, sh, st);
     }
-    return small ? launch_tile<T, WHAT, 64>(A, B, out, ptr, slot, sh, fast, st)
-                 : launch_tile<T, WHAT, 128>(A, B, out, ptr, slot, sh, fast, st);
+    return small ? launch_tile<T, WHAT, 64>(A, B, out, ptr, slot, sh, st)
+                 : launch_tile<T, WHAT, 128>(A, B, out, ptr, slot, sh, st);
 }
 template <Product WHAT>
 int experts_entry(const void *A, const void *B, void *out, int dtype, const int *ptr, const int *slot, int k, int M,

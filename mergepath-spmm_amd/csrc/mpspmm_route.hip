@@ -401,7 +401,7 @@ __device__ __forceinline__ void route_token(const T *__restrict__ row, bool live
     {
         const int valid = live ? sh.E - lane * IPL : 0;
         if (valid >= IPL) {
-            load_vec<T, IPL, false>(l, row + lane * IPL, valid);
+            load_vec<T, IPL>(l, row + lane * IPL, valid);
         } else {
 #pragma unroll
             for (int i = 0; i < IPL; ++i) l[i] = i < valid ? (float)row[lane * IPL + i] : minus_inf;
@@ -429,7 +429,7 @@ __device__ __forceinline__ void route_token(const T *__restrict__ row, bool live
         }
     } else {
         float b[IPL];
-        load_vec<float, IPL, false>(b, bias + (bias ? lane * IPL : 0), bias ? sh.E - lane * IPL : 0);
+        load_vec<float, IPL>(b, bias + (bias ? lane * IPL : 0), bias ? sh.E - lane * IPL : 0);
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < IPL; ++i) {
@@ -810,7 +810,7 @@ __global__ __launch_bounds__(kRouteBlock) void route_backward_kernel(const T *__
 // Y[t] = base[t] + sum_j w[t, j] Z[pos[t, j]]: one lane per 16 bytes of a row
 // of Y.  Bound by the bytes of Z and Y; the k rows of a token are asked for
 // together, four at a time.
-template <typename T, bool ALIGNED>
+template <typename T>
 __global__ __launch_bounds__(256) void combine_kernel(const T *__restrict__ Z, const int *__restrict__ pos,
                                                       const float *__restrict__ weight, const T *base, T *Y, int T_,
                                                       int k, int M, int N, int per_row)
@@ -822,7 +822,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const T *__restrict__ Z, c
     const int col = (int)(item - t * per_row) * V;
     const int valid = N - col;
     float acc[V];
-    if (base) load_vec<T, V, ALIGNED>(acc, base + t * N + col, valid);
+    if (base) load_vec<T, V>(acc, base + t * N + col, valid);
     else {
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = 0.0f;
@@ -838,7 +838,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const T *__restrict__ Z, c
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (p[j] >= 0) load_vec<T, V, ALIGNED>(z[j], Z + (long long)p[j] * N + col, valid);
+            if (p[j] >= 0) load_vec<T, V>(z[j], Z + (long long)p[j] * N + col, valid);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (p[j] >= 0) {
@@ -846,14 +846,14 @@ __global__ __launch_bounds__(256) void combine_kernel(const T *__restrict__ Z, c
                 for (int i = 0; i < V; ++i) acc[i] = __builtin_fmaf(w[j], z[j][i], acc[i]);
             }
     }
-    store_vec<T, V, ALIGNED>(Y + t * N + col, acc, valid);
+    store_vec<T, V>(Y + t * N + col, acc, valid);
 }
 
 // L lanes per place, a wavefront or for narrow rows less: they read the row of Z
 // and the token's row of dY, write the row of dZ and the product of the two
 // rows.  Places are in order, so Z and dZ stream; the k reads of a row of dY meet
 // in the caches.
-template <typename T, int L, bool ALIGNED>
+template <typename T, int L>
 __global__ __launch_bounds__(256) void combine_backward_kernel(const T *__restrict__ dY, const T *__restrict__ Z,
                                                                const float *__restrict__ weight,
                                                                const int *__restrict__ expert_ptr, int E,
@@ -881,8 +881,8 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T *__restri
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int col = first + u * L * V;
-            load_vec<T, V, ALIGNED>(y[u], y_row + col, routed ? N - col : 0);
-            load_vec<T, V, ALIGNED>(z[u], z_row + col, routed && dweight ? N - col : 0);
+            load_vec<T, V>(y[u], y_row + col, routed ? N - col : 0);
+            load_vec<T, V>(z[u], z_row + col, routed && dweight ? N - col : 0);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -892,7 +892,7 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T *__restri
                 dot = __builtin_fmaf(y[u][i], z[u][i], dot);
                 y[u][i] = routed ? y[u][i] * w : 0.0f;
             }
-            if (col < N) store_vec<T, V, ALIGNED>(out + col, y[u], N - col);
+            if (col < N) store_vec<T, V>(out + col, y[u], N - col);
         }
     }
     if (dweight && known) {
@@ -986,14 +986,8 @@ int launch_combine(const void *Z, const int *pos, const float *weight, const voi
     const int per_row = ceil_div(N, 16 / (int)sizeof(T));
     const long long blocks = ((long long)T_ * per_row + 255) / 256;
     if (blocks > INT_MAX) return MPS_ERR_UNSUPPORTED;
-    const bool fast = rows_of_16(Z, N, sizeof(T)) && rows_of_16(Y, N, sizeof(T)) && rows_of_16(base, N, sizeof(T));
-#define MPS_LAUNCH_COMBINE(ALIGNED)                                                                               \
-    hipLaunchKernelGGL((combine_kernel<T, ALIGNED>), grid_of(blocks), dim3(256), 0, st,                           \
-                       static_cast<const T *>(Z), pos, weight, static_cast<const T *>(base), static_cast<T *>(Y), \
-                       T_, k, M, N, per_row)
-    if (fast) MPS_LAUNCH_COMBINE(true);
-    else MPS_LAUNCH_COMBINE(false);
-#undef MPS_LAUNCH_COMBINE
+    hipLaunchKernelGGL((combine_kernel<T>), grid_of(blocks), dim3(256), 0, st, static_cast<const T *>(Z), pos, weight,
+                       static_cast<const T *>(base), static_cast<T *>(Y), T_, k, M, N, per_row);
     MPS_HIP_TRY(hipGetLastError());
     return MPS_OK;
 }
@@ -1002,22 +996,17 @@ template <typename T>
 int launch_combine_backward(const void *dY, const void *Z, const float *weight, const int *expert_ptr, int E,
                             const int *slot, void *dZ, float *dweight, int k, int M, int N, hipStream_t st)
 {
-    const bool fast = rows_of_16(dY, N, sizeof(T)) && rows_of_16(Z, N, sizeof(T)) && rows_of_16(dZ, N, sizeof(T));
     // as many lanes as a row has chunks (34076 places of 39 columns bf16: 10.6 us a call, 29.7 with 64)
     const int chunks = ceil_div(N, 16 / (int)sizeof(T));
-#define MPS_LAUNCH_COMBINE(L, ALIGNED)                                                                             \
-    hipLaunchKernelGGL((combine_backward_kernel<T, L, ALIGNED>), grid_of(ceil_div(M, 256 / L)), dim3(256), 0, st,  \
-                       static_cast<const T *>(dY), static_cast<const T *>(Z), weight, expert_ptr, E, slot,         \
+#define MPS_LAUNCH_LANES(L)                                                                                            \
+    hipLaunchKernelGGL((combine_backward_kernel<T, L>), grid_of(ceil_div(M, 256 / L)), dim3(256), 0, st,               \
+                       static_cast<const T *>(dY), static_cast<const T *>(Z), weight, expert_ptr, E, slot,             \
                        static_cast<T *>(dZ), dweight, k, M, N)
-#define MPS_LAUNCH_LANES(L)                     \
-    if (fast) MPS_LAUNCH_COMBINE(L, true);      \
-    else MPS_LAUNCH_COMBINE(L, false)
-    if (chunks <= 8) { MPS_LAUNCH_LANES(8); }
-    else if (chunks <= 16) { MPS_LAUNCH_LANES(16); }
-    else if (chunks <= 32) { MPS_LAUNCH_LANES(32); }
-    else { MPS_LAUNCH_LANES(64); }
+    if (chunks <= 8) MPS_LAUNCH_LANES(8);
+    else if (chunks <= 16) MPS_LAUNCH_LANES(16);
+    else if (chunks <= 32) MPS_LAUNCH_LANES(32);
+    else MPS_LAUNCH_LANES(64);
 #undef MPS_LAUNCH_LANES
-#undef MPS_LAUNCH_COMBINE
     MPS_HIP_TRY(hipGetLastError());
     return MPS_OK;
 }

@@ -49,22 +49,15 @@ inline bool rows_of_16(const void *p, long long row_elems, int elem_bytes)
     return aligned_to(p, 16) && row_elems * elem_bytes % 16 == 0;
 }
 
-// V elements of T at an address that is only aligned to the element.
+// V elements of T at an address that is only aligned to the element, of which
+// `valid` exist.  Global memory takes one wide access at any such address, so that
+// rows of whole 16 bytes have no variant of their own: it was the same instructions.
 template <typename T, int V>
-struct Vec {
-    typedef T type __attribute__((ext_vector_type(V)));
-};
-template <typename T>
-struct Vec<T, 1> {
-    using type = T;
-};
-template <typename T, int V, bool ALIGNED>
 __device__ __forceinline__ void load_vec(float (&out)[V], const T *p, int valid)
 {
     if (valid >= V) {
         T raw[V];
-        if constexpr (ALIGNED) __builtin_memcpy(raw, __builtin_assume_aligned(p, V * sizeof(T)), V * sizeof(T));
-        else __builtin_memcpy(raw, __builtin_assume_aligned(p, sizeof(T)), V * sizeof(T));
+        __builtin_memcpy(raw, __builtin_assume_aligned(p, sizeof(T)), V * sizeof(T));
 #pragma unroll
         for (int i = 0; i < V; ++i) out[i] = (float)raw[i];
     } else {
@@ -72,15 +65,14 @@ __device__ __forceinline__ void load_vec(float (&out)[V], const T *p, int valid)
         for (int i = 0; i < V; ++i) out[i] = i < valid ? (float)p[i] : 0.0f;
     }
 }
-template <typename T, int V, bool ALIGNED>
+template <typename T, int V>
 __device__ __forceinline__ void store_vec(T *p, const float (&v)[V], int valid)
 {
     if (valid >= V) {
         T raw[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) raw[i] = (T)v[i];
-        if constexpr (ALIGNED) __builtin_memcpy(__builtin_assume_aligned(p, V * sizeof(T)), raw, V * sizeof(T));
-        else __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), raw, V * sizeof(T));
+        __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), raw, V * sizeof(T));
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -115,13 +107,13 @@ __device__ __forceinline__ float4v mma(uint4v p, uint4v q, float4v acc)
 }
 
 // 16 bytes from p, of which `valid` elements exist; zeros for the others.
-template <typename T, bool ALIGNED>
+template <typename T>
 __device__ __forceinline__ uint4v load_chunk(const T *p, int valid)
 {
     constexpr int V = 16 / sizeof(T);
     uint4v v = {0, 0, 0, 0};
     if (valid >= V) {
-        __builtin_memcpy(&v, __builtin_assume_aligned(p, ALIGNED ? 16 : sizeof(T)), 16);
+        __builtin_memcpy(&v, __builtin_assume_aligned(p, sizeof(T)), 16);
     } else if (valid > 0) {
         T part[V];
 #pragma unroll
