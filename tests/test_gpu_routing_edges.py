@@ -437,3 +437,52 @@ def test_route_backward_against_differences_of_the_kernel(r, dev, score, renorma
     assert same.sum() >= T // 4
     slope = ((up.weight.cpu().double() - down.weight.cpu().double()) * dw.double()).sum(1) / (2 * h)
     assert ((grad * v.double()).sum(1) - slope)[same].abs().max() < 0.014
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Captured
+# ---------------------------------------------------------------------------------------------------------------------
+
+def test_two_captured_graphs_with_workspaces(r, dev):
+    """Long routings, their gradients and adapters, whose calls take workspaces, in two graphs: replayed in turn, with
+    eager calls between, each gives what the eager calls give, bit for bit."""
+    T, E, k, D = 3000, 40, 4, 64
+    t = torch.float16
+    A, B = normal(2, 3, 24, D, t=t, scale=0.125).to(dev), normal(3, 3, D, 24, t=t, scale=0.3).to(dev)
+    bias = normal(4, E, scale=0.1).to(dev)
+    adapter = (torch.arange(T, dtype=torch.int32, device=dev) % 4).view(T, 1)
+    options = dict(score="sigmoid", renormalise=True)
+
+    def layer(x, scores):
+        m = r.route(scores, k, bias=bias, groups=4, top_groups=2, group_score="top2", **options)
+        z = x[m.slot.long() // k]
+        g = r.combine_backward(x, z, m.weight, m.expert_ptr, m.slot)
+        ds = r.route_backward(scores, m.expert, g["dweight"], **options)
+        ptr, row, _ = r.columns(adapter, 3)
+        return r.adapters_mm(x, A, B, None, ptr, row, base=r.combine(z, m.pos, m.weight)), ds, g["dZ"], *m
+
+    def masked(seed):
+        return torch.from_numpy(masked_groups(seed, T, E, 4))
+
+    inputs = [(torch.zeros(T, D, dtype=t, device=dev), torch.zeros(T, E, device=dev)) for _ in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for a in inputs:
+            layer(*a)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, captured = [torch.cuda.CUDAGraph() for _ in inputs], []
+    for graph, a in zip(graphs, inputs):
+        with torch.cuda.graph(graph):
+            captured.append(layer(*a))
+    for n in range(3):
+        for i, a in enumerate(inputs):
+            a[0].copy_(normal(10 * n + i, T, D, t=t))
+            a[1].copy_(masked(10 * n + i))
+        for graph in graphs:
+            graph.replay()
+        for graph, got, a in zip(graphs, captured, inputs):
+            ref = layer(*a)
+            torch.cuda.synchronize()
+            for x, y in zip(got, ref):
+                assert torch.equal(x, y)
