@@ -642,7 +642,8 @@ int mps_nzsplit_spmm_f32(const int *d_col_idx, const float *d_val, const float *
  *               has no expert.
  * Conventions beside those at the top of this file: dense data may be fp32,
  * fp16 or bf16 (mps_dtype) and needs only its natural alignment (16-byte
- * aligned matrices with rows of whole 16 bytes are faster); sums are held in
+ * aligned matrices with rows of whole 16 bytes are faster: the products of the
+ * experts have kernels of their own for them); sums are held in
  * fp32 and rounded once; calls only launch kernels (no allocation, copy,
  * memset or synchronisation), so they can be captured; results are the same
  * bits from run to run (no atomics on results).  Every index that a kernel
@@ -674,7 +675,8 @@ typedef struct mps_route_options {
  *   group; a sum of two is -inf where the group has no two experts), and among their experts the k with the largest c are chosen
  *   (ties: the lower expert), in descending order of c;
  *   weight = scale * s, or scale * s / (sum of the chosen s).
- * Without a bias c orders as l does, and l itself is compared.  An expert with
+ * Without a bias and without sums of two over groups c orders as l does, and l
+ * itself is compared.  An expert with
  * l = -inf or a bias of -inf is never chosen; slots that find no expert hold
  * -1 and weight 0, also where renormalised.  Else a NaN counts as the largest
  * value, as does what is computed from one, so that it shows in the weights.

@@ -187,6 +187,10 @@ __global__ __launch_bounds__(64 * kWaves) void adapters_expand_kernel(const floa
     const T *b_of = B + (size_t)max(t.expert, 0) * sh.N * sh.R;
     // Stores are counted with the loads, in order, so that a load behind a store
     // waits for it: the next 64 columns are asked for before these are stored.
+    // The two sets of operands change places by a copy, though, for which the
+    // compiler waits until all of a turn's loads and stores are done, so that only
+    // the stores' issue overlaps with the loads.  8192 tokens, rank 64, 4096 columns
+    // fp16: 55 of the 91 us in all.
     // (Ranks over 64 have no registers for two, and one turn.)
     struct Operands {
         uint4v p[STEPS][4], y[MT][PER == 1 ? 4 : 2];
@@ -265,6 +269,11 @@ AdaptersShape make_shape(int T, int E, int R, int K, int N)
 {
     int padded = 16;
     while (padded < R) padded *= 2;
+    // Taller tiles from 128 tokens an adapter on.  Measured with and without, K = N =
+    // 4096 fp16, us: rank 64, 12 adapters: 683 tokens each 91 / 106, 512: 83 / 83, 256:
+    // 72 / 54, 128: 68 / 43, 64: 46 / 28; 4 adapters: 512: 72 / 43; rank 256, 4 adapters:
+    // 512: 281 / 135; rank 16, 12 adapters: 512: 51 / 44.  So they gain at long segments of
+    // many adapters alone, where the short tiles fill the GPU several times over.
     AdaptersShape sh{T, E, R, K, N, padded, 1, K, T >= 128LL * E};
     // Parts of the sum over K: about 512 workgroups, each with at least 256 of K.
     const long long tiles = num_row_tiles(T, E < T ? E : T, sh.tall ? 64 : 16);
@@ -326,8 +335,9 @@ int launch_adapters(const void *X_, const void *A_, const void *B_, const float 
 #define MPS_EXPAND(RANK)                                                                                         \
     return sh.tall && RANK <= 2 ? launch_expand<T, RANK, RANK <= 2 ? 2 : 1>(V, B, scale, base, Y, ptr, row_of, sh, st) \
                                   : launch_expand<T, RANK, 1>(V, B, scale, base, Y, ptr, row_of, sh, st)
-    // Tiles of 32 tokens: 8192 tokens, rank 64, 4096 columns take 92 us in all, 106 with 16, 156 with 64, which
-    // leave one wavefront a SIMD.
+    // Tiles of 32 tokens: 8192 tokens, rank 64, 4096 columns take 91 us in all, 106 with 16, 156 with 64, which
+    // leave one wavefront a SIMD.  Ranks from 65 to 256 share one kernel, with the matrix work of 256: 12 adapters of
+    // 512 tokens take 83 us at rank 64, 229 at 128, 453 at 256.
     if (sh.R <= 32) MPS_EXPAND(1);
     if (sh.R <= 64) MPS_EXPAND(2);
     MPS_EXPAND(8);

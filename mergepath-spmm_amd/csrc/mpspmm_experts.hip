@@ -273,8 +273,8 @@ __global__ __launch_bounds__(kThreads, 2) void experts_tile_kernel(const T *__re
 // from memory into LDS, two of them in turn: while the matrix instructions work
 // on one, the other is on its way.  Measured, 256 x 256 tiles, fp16: 1202 TFLOP/s
 // for one expert of 8192 x 8192 x 8192 (a library product: 1414), 897 for 64
-// experts of 768 rows, 1408 x 2048 (a last tile of half the columns), 840 where
-// their rows are uneven.  Four stages of one matrix step, for requests three
+// experts of 768 rows, 1408 x 2048 (a last tile of half the columns), 820 - 840
+// where their rows are uneven.  Four stages of one matrix step, for requests three
 // ahead, and sums that begin at another place in every column tile gave nothing:
 // neither the way from memory nor its channels bound it.
 //   PP, QP  panels of S in the tile's columns and rows
@@ -632,7 +632,14 @@ int launch_experts(const void *A, const void *B, void *out, const int *ptr, cons
                       rows_of_16(out, WHAT == kForward ? N : K, sizeof(T));
     if constexpr (WHAT == kForward) {
         // Few rows an expert: the tiles below would be nearly empty and their workgroups few (32 tokens, 6 of 64 experts,
-        // 2048 x 1024 bf16: 59 us, 62 - 80 with tiles of 128).
+        // 2048 x 1024 bf16: 56 - 59 us, 62 - 80 with tiles of 128).  Measured on experts of uneven length, K = 2048, us
+        // with 16 rows / 32 rows / the tiles below, by the mean rows of an expert:
+        //   64 of 1408 columns, bf16   4: 72 / 68 / 89   9: 93 / 87 / 97   16: 114 / 97 / 96   24: 136 / 111 / 96
+        //                       fp32   8: 180 / 217 / 445   16: 242 / 258 / 469   25: 303 / 300 / 469   48: 476 / 431 / 472
+        //   32 of 1024 columns, bf16   4: 33 / 37 / 29    8: 38 / 38 / 30    24: 54 / 51 / 36
+        //                       fp32   8: 78 / 108 / 74   24: 121 / 146 / 97
+        // Where the tiles below are those of 64 they are ahead from 4 rows on, those of 128 from 16 (bf16) or 64 (fp32):
+        // 24 lies between.
         if (M <= 8LL * E) return launch_few<T, 1>(A, B, out, ptr, slot, sh, st);
         if (M <= 24LL * E) return launch_few<T, 2>(A, B, out, ptr, slot, sh, st);
     }
@@ -640,6 +647,13 @@ int launch_experts(const void *A, const void *B, void *out, const int *ptr, cons
     const long long tiles = WHAT == kWeights ? (long long)E * ceil_div(N, 128) * ceil_div(K, 128)
                                              : ((long long)M / 128 + (E < M ? E : M)) * ceil_div(WHAT == kForward ? N : K, 128);
     const bool small = tiles < 512;
+    // 256 x 256 tiles from 384 rows on.  Measured on uneven experts, bf16, us with them / with tiles of 128 or 64:
+    //   product, 32 of 1024 x 2048    256: 63 / 74    384: 108 / 81    512: 110 / 110   768: 122 / 152
+    //            64 of 1408 x 2048    256: 169 / 164  384: 223 / 220   512: 259 / 272   768: 333 / 385
+    //   dX,      64 of 1408 x 2048    128: 122 / 126  256: 162 / 181   384: 208 / 236   768: 361 / 413
+    //   dW,      32 of 1024 x 2048     96: 60 / 70    256: 81 / 95     384: 96 / 111    768: 149 / 176
+    // The rule looks at the rows alone.  Narrow matrices of few experts make few such tiles, and dW is never cut along
+    // its places: 65536 rows, 2 experts of 64 x 64: dW 526 / 242, 16 of 256 x 512: dW 110 / 44, product 43 / 35.
     // offsets of 32 bits inside X or dY and inside the matrix of an expert
     const long long far = INT_MAX / (long long)sizeof(T);
     const bool near = (long long)M * (WHAT == kForward ? K : N) <= far && (long long)N * K <= far &&
