@@ -519,7 +519,7 @@ int launch_stream(const void *A, const void *B, void *out, const int *ptr, const
     sh.col_tiles = ceil_div(WHAT == kForward ? sh.N : sh.K, PP * S);
     sh.row_tiles = ceil_div(sh.N, QP * S);
     const long long others = WHAT == kWeights ? (long long)sh.E * sh.row_tiles : num_row_tiles(sh.M, sh.E, QP * S);
-    if (!fits_launch(others * sh.col_tiles, 64 * WP * WQ)) return MPS_ERR_UNSUPPORTED;
+    if (!fits_launch(others, sh.col_tiles, 64 * WP * WQ)) return MPS_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((experts_stream_kernel<T, WHAT, S, PP, QP, WP, WQ>), dim3((unsigned)(others * sh.col_tiles)),
                        dim3(64 * WP * WQ), 0, st, static_cast<const T *>(A), static_cast<const T *>(B),
                        static_cast<T *>(out), ptr, slot, sh);
@@ -600,9 +600,9 @@ template <typename T, int MT>
 int launch_few(const void *X, const void *W, void *Y, const int *ptr, const int *slot, ExpertsShape sh, hipStream_t st)
 {
     sh.col_tiles = ceil_div(sh.N, 16 * kFewColumns);
-    const long long blocks = num_row_tiles(sh.M, sh.E, 16 * MT) * sh.col_tiles;
-    if (!fits_launch(blocks, 64 * kFewWaves)) return MPS_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((experts_few_kernel<T, MT>), dim3((unsigned)blocks), dim3(64 * kFewWaves), 0, st,
+    const long long tiles = num_row_tiles(sh.M, sh.E, 16 * MT);
+    if (!fits_launch(tiles, sh.col_tiles, 64 * kFewWaves)) return MPS_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((experts_few_kernel<T, MT>), dim3((unsigned)(tiles * sh.col_tiles)), dim3(64 * kFewWaves), 0, st,
                        static_cast<const T *>(X), static_cast<const T *>(W), static_cast<T *>(Y), ptr, slot, sh);
     MPS_HIP_TRY(hipGetLastError());
     return MPS_OK;
@@ -614,7 +614,7 @@ int launch_tile(const void *A, const void *B, void *out, const int *ptr, const i
     sh.col_tiles = ceil_div(WHAT == kForward ? sh.N : sh.K, S);
     sh.row_tiles = ceil_div(sh.N, S);
     const long long others = WHAT == kWeights ? (long long)sh.E * sh.row_tiles : num_row_tiles(sh.M, sh.E, S);
-    if (!fits_launch(others * sh.col_tiles, kThreads)) return MPS_ERR_UNSUPPORTED;
+    if (!fits_launch(others, sh.col_tiles, kThreads)) return MPS_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((experts_tile_kernel<T, WHAT, S>), dim3((unsigned)(others * sh.col_tiles)), dim3(kThreads), 0, st,
                        static_cast<const T *>(A), static_cast<const T *>(B), static_cast<T *>(out), ptr, slot, sh);
     MPS_HIP_TRY(hipGetLastError());
@@ -644,9 +644,8 @@ int launch_experts(const void *A, const void *B, void *out, const int *ptr, cons
         if (M <= 24LL * E) return launch_few<T, 2>(A, B, out, ptr, slot, sh, st);
     }
     // Tiles of 64 where tiles of 128 would leave compute units without one.
-    const long long tiles = WHAT == kWeights ? (long long)E * ceil_div(N, 128) * ceil_div(K, 128)
-                                             : ((long long)M / 128 + (E < M ? E : M)) * ceil_div(WHAT == kForward ? N : K, 128);
-    const bool small = tiles < 512;
+    const long long others = WHAT == kWeights ? (long long)E * ceil_div(N, 128) : (long long)M / 128 + (E < M ? E : M);
+    const bool small = others < 512 && others * ceil_div(WHAT == kForward ? N : K, 128) < 512;
     // 256 x 256 tiles from 384 rows on.  Measured on uneven experts, bf16, us with them / with tiles of 128 or 64:
     //   product, 32 of 1024 x 2048    256: 63 / 74    384: 108 / 81    512: 110 / 110   768: 122 / 152
     //            64 of 1408 x 2048    256: 169 / 164  384: 223 / 220   512: 259 / 272   768: 333 / 385

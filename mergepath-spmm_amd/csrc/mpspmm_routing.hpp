@@ -40,8 +40,12 @@ inline dim3 grid_of(long long blocks)
 }
 __device__ __forceinline__ long long block_number() { return (long long)blockIdx.y * kGridRow + blockIdx.x; }
 
-// Whether so many workgroups fit one dimension.
-inline bool fits_launch(long long blocks, int threads) { return blocks <= 0xFFFFFFFFll / threads; }
+// Whether a x b workgroups fit one dimension; a b may be beyond 64 bits.
+inline bool fits_launch(long long a, long long b, int threads)
+{
+    const long long most = 0xFFFFFFFFll / threads;
+    return a <= most && b <= most && a * b <= most;
+}
 
 // A matrix whose rows are loaded 16 bytes at a time: aligned base, rows of whole 16 bytes.
 inline bool rows_of_16(const void *p, long long row_elems, int elem_bytes)

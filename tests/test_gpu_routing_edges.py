@@ -302,8 +302,9 @@ def test_combine_of_many_rows(r, dev):
     """More than 2^32 chunks of 16 bytes in the result."""
     N, t = 1024, torch.float16
     T = (1 << 25) + 9
-    if torch.cuda.mem_get_info(dev)[0] < 100 << 30:
-        torch.cuda.empty_cache()
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(dev)[0] < 80 << 30:
+        pytest.skip("the result takes 64 GB")
     Z = normal(1, 40, N, t=t).to(dev)
     pos = (torch.arange(T, device=dev) % 41).int().view(T, 1)
     pos[pos == 40] = -1

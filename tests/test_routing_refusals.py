@@ -160,3 +160,6 @@ def test_experts_of_more_tiles_than_a_launch_holds(L):
     assert L.mps_experts_mm(P, P, P, 2, P, None, 1, 1 << 30, 1 << 10, 1 << 20, 8, None) == UNSUPPORTED
     assert L.mps_experts_mm_dx(P, P, P, 1, P, 64, 1 << 24, 1, 1, None) == UNSUPPORTED
     assert L.mps_experts_mm(P, P, P, 1, P, None, 1, 64, 2 ** 31 - 1, 1, 1, None) == UNSUPPORTED
+    # 2^66 tiles of 64 x 64, less 2^44
+    n = (1 << 29) - 64
+    assert L.mps_experts_mm_dw(P, P, P, 0, P, None, 1, 64, 1 << 20, n, n, None) == UNSUPPORTED
