@@ -672,13 +672,14 @@ typedef struct mps_route_options {
  *   s = softmax(l) over all E experts, or sigmoid(l);
  *   c = s + d_bias (d_bias: float[E] or NULL), in the precision of 64 bits;
  *   the top_groups groups with the largest group score stay (ties: the lower
- *   group; a sum of two is -inf where the group has no two experts), and among their experts the k with the largest c are chosen
+ *   group; a sum of two is -inf where the group has fewer than two experts that
+ *   can be chosen), and among their experts the k with the largest c are chosen
  *   (ties: the lower expert), in descending order of c;
  *   weight = scale * s, or scale * s / (sum of the chosen s).
  * Without a bias and without sums of two over groups c orders as l does, and l
- * itself is compared.  An expert with
- * l = -inf or a bias of -inf is never chosen; slots that find no expert hold
- * -1 and weight 0, also where renormalised.  Else a NaN counts as the largest
+ * itself is compared.  An expert with l = -inf or a bias of -inf is never
+ * chosen; slots that find no expert hold -1 and weight 0, also where
+ * renormalised.  Else a NaN counts as the largest
  * value, as does what is computed from one, so that it shows in the weights.
  * d_expert_ptr, d_slot, d_pos: all three or all NULL (the rows alone).
  * The workspace is needed for the columns only. */

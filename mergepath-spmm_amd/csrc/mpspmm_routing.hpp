@@ -32,7 +32,8 @@ inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // A launch holds fewer than 2^32 threads in a dimension, which a wavefront for
 // every one of 2^26 tokens reaches; of more only the rest is run, without an
-// error.  More workgroups than kGridRow go into rows of a second dimension.  Numbers from `blocks` on occur; a kernel gives them nothing.
+// error.  More workgroups than kGridRow go into rows of a second dimension.
+// Numbers from `blocks` on occur then; a kernel has nothing to do for them.
 constexpr int kGridRow = 1 << 22;
 inline dim3 grid_of(long long blocks)
 {
